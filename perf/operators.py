@@ -1,0 +1,378 @@
+"""Timing cases of the vocabulary operators: the last steps of a captioner (or any model over a vocabulary).
+
+Four operators: drawing tokens with temperature, top-k, top-p and min-p from given uniforms; the k largest
+entries of each row with the row's log-normaliser (the record a teacher leaves); distillation from such a
+record, forward and backward; and the product of activations with an 8-bit weight (e4m3, one power-of-two
+scale for each row and block of 128).  With ``own`` false ``run`` computes them from elementary torch
+operations; with ``own`` true it calls this repository's entry points.
+"""
+import math
+
+import numpy as np
+import torch
+
+own = False
+
+DTYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+BYTES = {"f32": 4, "bf16": 2, "f16": 2}
+BLOCK = 128   # entries that share a scale in an 8-bit operand
+
+
+def _hip():
+    import importlib
+    return importlib.import_module("image-captioning-through-rl_amd.hipabi")
+
+
+def listed():
+    return [
+        # one caption decoded alone: a single row of the 10 000-word vocabulary, all of the usual filters on
+        dict(name="sample_one", op="sample", n=1, v=10000, pad=0, dtype="f32", per_row=False,
+             temperature=0.8, top_k=50, top_p=0.95, min_p=0.0),
+        # a training minibatch's rows (512) drawn from the nucleus; the logits are the left columns of a wider
+        # matrix, as in the rollout, where the recurrent product stands beside them
+        dict(name="sample_nucleus", op="sample", n=512, v=10000, pad=2288, dtype="f32", per_row=False,
+             temperature=1.0, top_k=0, top_p=0.9, min_p=0.0),
+        # a serving batch over a large vocabulary, every request with its own settings (some greedy, some open)
+        dict(name="sample_requests", op="sample", n=64, v=131072, pad=0, dtype="bf16", per_row=True,
+             temperature=1.0, top_k=0, top_p=1.0, min_p=0.0),
+        # an odd vocabulary: no row but the first is aligned
+        dict(name="sample_odd", op="sample", n=333, v=50257, pad=0, dtype="f16", per_row=False,
+             temperature=1.3, top_k=0, top_p=1.0, min_p=0.05),
+        # a few teacher rows recorded while serving
+        dict(name="record_few", op="record", n=64, v=32000, pad=0, dtype="bf16", k=16, temperature=1.0),
+        # the teacher's record for a whole minibatch: 512 captions x 19 positions
+        dict(name="record_minibatch", op="record", n=9728, v=10000, pad=0, dtype="f32", k=64, temperature=2.0),
+        # validation loss of a small batch: forward only
+        dict(name="distill_validate", op="distill", n=64, v=10000, pad=0, dtype="f32", k=8, temperature=1.0,
+             tail=True, calls="forward", idle=0.0),
+        # a training minibatch (512 captions x 19 positions, the positions after <END> idle): loss and gradient at once
+        dict(name="distill_minibatch", op="distill", n=9728, v=10000, pad=0, dtype="f32", k=64, temperature=2.0,
+             tail=True, calls="fused", idle=0.2),
+        # a large vocabulary in bf16: the forward pass first, the gradient later from what it kept
+        dict(name="distill_large", op="distill", n=512, v=131072, pad=0, dtype="bf16", k=128, temperature=1.0,
+             tail=False, calls="two", idle=0.05),
+        # the vocabulary product of one caption's step
+        dict(name="linear8_one", op="linear8", m=1, n=10000, k=512, dtype="f32", out="f32", bias=True),
+        # the vocabulary product of a minibatch's step
+        dict(name="linear8_step", op="linear8", m=512, n=10000, k=512, dtype="f32", out="f32", bias=True),
+        # 4096 positions against a 32 000-word vocabulary at width 2048
+        dict(name="linear8_large", op="linear8", m=4096, n=32000, k=2048, dtype="bf16", out="bf16", bias=False),
+    ]
+
+
+def _log_int(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def draw(rng):
+    op = rng.choice(["sample", "sample", "record", "distill", "distill", "linear8"])
+    dtype = rng.choice(["f32", "bf16", "f16"])
+    if op == "linear8":
+        m, n, k = _log_int(rng, 1, 8192), _log_int(rng, 128, 32000), _log_int(rng, 64, 4096)
+        while 2 * m * n * k > 4e11 or m * n > 1 << 27:
+            m = max(1, m // 2)
+        return dict(op=op, m=m, n=n, k=k, dtype=dtype, out=rng.choice(["f32", "bf16"]), bias=rng.random() < 0.5)
+    v = _log_int(rng, 100, 151000)
+    n = _log_int(rng, 1, 4096)
+    while n * v > 1 << 26:
+        n = max(1, n // 2)
+    pad = rng.choice([0, 0, 3, 64])
+    case = dict(op=op, n=n, v=v, pad=pad, dtype=dtype)
+    if op == "sample":
+        case.update(per_row=rng.random() < 0.3, temperature=round(rng.uniform(0.3, 1.6), 3),
+                    top_k=rng.choice([0, 0, 1, 5, 40, 200]), top_p=round(rng.choice([1.0, rng.uniform(0.3, 0.99)]), 3),
+                    min_p=round(rng.choice([0.0, 0.0, rng.uniform(0.005, 0.3)]), 4))
+    else:
+        case.update(k=min(v, _log_int(rng, 1, 512)), temperature=round(rng.uniform(0.5, 4.0), 3))
+    if op == "distill":
+        case.update(tail=rng.random() < 0.6, calls=rng.choice(["forward", "fused", "two"]),
+                    idle=rng.choice([0.0, 0.3]))
+    return case
+
+
+# ---------------------------------------------------------------------------------------------- inputs
+def _logits(n, v, pad, dtype, gen):
+    """Rows like a trained network's: a bulk of unlikely words and a few likely ones."""
+    x = torch.randn(n, v + pad, device="cuda", generator=gen) * 2.0
+    likely = torch.randint(0, v, (n, 1), device="cuda", generator=gen)
+    likely = (likely + torch.arange(24, device="cuda") * (v // 24)) % v   # no word twice: the sums have one order
+    x.scatter_add_(1, likely, torch.rand(n, 24, device="cuda", generator=gen) * 9.0)
+    return x.to(DTYPES[dtype])[:, :v]
+
+
+def prepare(case, seed):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    s = dict(case=case)
+    if case["op"] == "linear8":
+        m, n, k = case["m"], case["n"], case["k"]
+        s["x"] = torch.tanh(torch.randn(m, k, device="cuda", generator=gen)).to(DTYPES[case["dtype"]])
+        w = (torch.rand(n, k, device="cuda", generator=gen) * 2.0 - 1.0) / math.sqrt(k)
+        s["bias"] = (torch.rand(n, device="cuda", generator=gen) - 0.5) * 0.1 if case["bias"] else None
+        # the weight as it is kept: e4m3 codes and a power-of-two scale for each row and block of 128
+        s["w_codes"], s["w_scale"] = _codes(w)
+        if own:
+            hip = _hip()
+            s["out"] = torch.empty(m, n, dtype=DTYPES[case["out"]], device="cuda")
+            s["x8"], s["w8"] = hip.fp8_pieces(m, k, w.device), hip.fp8_pieces(n, k, w.device)
+            hip.cut_fp8(w, *s["w8"])
+        return s
+    n, v = case["n"], case["v"]
+    s["logits"] = _logits(n, v, case["pad"], case["dtype"], gen)
+    if case["op"] == "sample":
+        s["uniforms"] = torch.rand(n, device="cuda", generator=gen, dtype=torch.float64)
+        if case["per_row"]:
+            pick = torch.rand(4, n, device="cuda", generator=gen)
+            r = torch.rand(4, n, device="cuda", generator=gen)
+            s["temperature"] = torch.where(pick[0] < 0.1, torch.zeros_like(r[0]), 0.5 + r[0])
+            s["top_k"] = torch.where(pick[1] < 0.4, torch.zeros_like(r[1]), 1 + r[1] * 200).to(torch.int32)
+            s["top_p"] = torch.where(pick[2] < 0.4, torch.ones_like(r[2]), 0.5 + 0.49 * r[2])
+            s["min_p"] = torch.where(pick[3] < 0.6, torch.zeros_like(r[3]), 0.2 * r[3])
+        else:
+            s.update({p: case[p] for p in ("temperature", "top_k", "top_p", "min_p")})
+        s["tokens"] = torch.empty(n, dtype=torch.int64, device="cuda")
+        s["log_prob"] = torch.empty(n, device="cuda")
+        return s
+    k = case["k"]
+    if case["op"] == "record":
+        s["values"] = torch.empty(n, k, device="cuda")
+        s["indices"] = torch.empty(n, k, dtype=torch.int64, device="cuda")
+        s["lse"] = torch.empty(n, device="cuda")
+        return s
+    # distillation: the teacher is near the student, and knows some words better
+    teacher = s["logits"].float() + torch.randn(n, v, device="cuda", generator=gen)
+    s["t_values"], s["t_indices"] = torch.topk(teacher, k, dim=1)
+    s["t_lse"] = torch.logsumexp(teacher.double() / case["temperature"], 1).float() if case["tail"] else None
+    s["weight"] = torch.rand(n, device="cuda", generator=gen) + 0.5
+    s["weight"][torch.rand(n, device="cuda", generator=gen) < case["idle"]] = 0.0
+    s["loss"] = torch.empty(n, device="cuda")
+    s["stats"] = torch.empty(n, 4, device="cuda")
+    if case["calls"] != "forward":
+        s["grad"] = torch.empty(n, v, dtype=s["logits"].dtype, device="cuda")
+    return s
+
+
+def work(case):
+    if case["op"] == "linear8":
+        m, n, k = case["m"], case["n"], case["k"]
+        return {"bytes": m * k * BYTES[case["dtype"]] + n * k + n * -(-k // BLOCK) + m * n * BYTES[case["out"]]
+                + (4 * n if case["bias"] else 0), "flops": 2 * m * n * k}
+    n, v, e = case["n"], case["v"], BYTES[case["dtype"]]
+    if case["op"] == "sample":
+        return {"bytes": n * v * e + 20 * n + (16 * n if case["per_row"] else 0), "flops": 2 * n * v}
+    k = case["k"]
+    if case["op"] == "record":
+        return {"bytes": n * v * e + 12 * n * k + 4 * n, "flops": 2 * n * v}
+    live = n * (1.0 - case["idle"])   # idle rows are not read; their gradient is zeros
+    grad = 0 if case["calls"] == "forward" else n * v * e
+    return {"bytes": int(live * (v * e + 12 * k)) + grad + 12 * n, "flops": int(4 * live * v)}
+
+
+# ---------------------------------------------------------------------------------------------- plain forms
+def _codes(x):
+    """x [rows, K] -> (e4m3 values of x / scale [rows, blocks, 128], scale [rows, blocks, 1]): the scale is the
+    smallest power of two that keeps the block's largest magnitude within 448, the type's largest value."""
+    rows, k = x.shape
+    blocks = -(-k // BLOCK)
+    x = torch.nn.functional.pad(x.float(), (0, blocks * BLOCK - k)).view(rows, blocks, BLOCK)
+    frac, exp = torch.frexp(x.abs().amax(2, keepdim=True))   # amax = frac 2^exp, frac in [0.5, 1)
+    exp = torch.where(frac == 0, torch.zeros_like(exp), torch.where(frac <= 0.875, exp - 9, exp - 8))
+    scale = torch.ldexp(torch.ones_like(frac), exp)
+    return (x / scale).to(torch.float8_e4m3fn).float(), scale
+
+
+def _plain_linear8(s):
+    case = s["case"]
+    codes, scale = _codes(s["x"])
+    x = (codes * scale).flatten(1)
+    w = (s["w_codes"] * s["w_scale"]).flatten(1)
+    out = x @ w.t()
+    if s["bias"] is not None:
+        out = out + s["bias"]
+    return out.to(DTYPES[case["out"]])
+
+
+def _column(p, n, dtype=torch.float64):
+    t = p if torch.is_tensor(p) else torch.full((n,), p, dtype=dtype, device="cuda")
+    return t.to(dtype).view(n, 1)
+
+
+def _plain_sample(s):
+    # 64 bits: a draw next to a border of the distribution has to fall on the same side everywhere
+    x = s["logits"].double()
+    n, v = x.shape
+    temperature, top_p, min_p = (_column(s[p], n) for p in ("temperature", "top_p", "min_p"))
+    top_k = _column(s["top_k"], n, torch.int64)
+    top_k = torch.where(temperature == 0, torch.ones_like(top_k), torch.where(top_k == 0, torch.full_like(top_k, v), top_k))
+    order = torch.sort(x, dim=1, descending=True, stable=True)   # ties: lowest index first
+    m = order.values[:, :1]
+    z = (order.values - m) / torch.where(temperature == 0, torch.ones_like(temperature), temperature)
+    w = torch.exp(z)
+    w = w * (torch.arange(v, device="cuda") < top_k)
+    cum = torch.cumsum(w, 1)
+    w = w * (cum - w < top_p * cum[:, -1:])          # the shortest prefix that holds top_p of the mass ...
+    w[:, 0] = 1.0                                    # ... and never fewer than one word
+    w = w * (w >= min_p)
+    w = torch.zeros_like(w).scatter_(1, order.indices, w)
+    cdf = torch.cumsum(w, 1)
+    total = cdf[:, -1:]
+    token = (cdf <= s["uniforms"].view(n, 1) * total).sum(1).clamp_(max=v - 1)
+    log_prob = torch.log(w.gather(1, token.view(n, 1)) / total).view(n)
+    return token, log_prob.float()
+
+
+def _plain_record(s):
+    case = s["case"]
+    x = s["logits"].float()
+    order = torch.sort(x, dim=1, descending=True, stable=True)
+    z = x / case["temperature"]
+    m = z.amax(1, keepdim=True)
+    lse = (m + torch.log(torch.exp(z - m).sum(1, keepdim=True))).view(-1)
+    return order.values[:, :case["k"]].contiguous(), order.indices[:, :case["k"]].contiguous(), lse
+
+
+def _plain_distill(s):
+    case = s["case"]
+    t = case["temperature"]
+    z = s["logits"].float() / t
+    m = z.amax(1, keepdim=True)
+    e = torch.exp(z - m)
+    total = e.sum(1, keepdim=True)
+    # the row's few numbers in 64 bits: what the record leaves over is a difference of nearly equal ones
+    tv = s["t_values"].double() / t
+    if case["tail"]:
+        t_lse = s["t_lse"].double().view(-1, 1)
+    else:
+        t_lse = torch.log(torch.exp(tv - tv.amax(1, keepdim=True)).sum(1, keepdim=True)) + tv.amax(1, keepdim=True)
+    q = torch.exp(tv - t_lse)
+    log_p = (z - m).gather(1, s["t_indices"]).double() - torch.log(total.double())
+    loss = (q * (tv - t_lse - log_p)).sum(1, keepdim=True)
+    mass = q.sum(1, keepdim=True)
+    ratio = torch.zeros_like(mass)
+    if case["tail"] and case["k"] < case["v"]:
+        rest = e.scatter(1, s["t_indices"], 0.0).sum(1, keepdim=True).double()
+        p_rest = rest / total.double()
+        q_rest = (1.0 - mass).clamp_(min=0.0)
+        gap = torch.where(q_rest > 0, q_rest * torch.log(q_rest / p_rest), torch.zeros_like(mass))
+        some = rest > 0
+        loss = loss + torch.where(some, gap, torch.zeros_like(gap))
+        ratio = torch.where(some, q_rest / p_rest, ratio)
+        mass = mass + torch.where(some, q_rest, torch.zeros_like(q_rest))
+    weight = s["weight"].double().view(-1, 1)
+    loss = (weight * loss).float().view(-1)
+    if case["calls"] == "forward":
+        return loss
+    p = e / total
+    grad = p * (weight / t * (mass - ratio)).float()
+    there = p.gather(1, s["t_indices"]).double() * mass - q
+    grad = grad.scatter(1, s["t_indices"], (weight / t * there).float())
+    return loss, grad.to(s["logits"].dtype)
+
+
+# ---------------------------------------------------------------------------------------------- one pass
+def run(s):
+    case = s["case"]
+    op = case["op"]
+    if not own:
+        return {"sample": _plain_sample, "record": _plain_record, "distill": _plain_distill,
+                "linear8": _plain_linear8}[op](s)
+    hip = _hip()
+    if op == "sample":
+        hip.sample_tokens_filtered(s["logits"], s["tokens"], 1, s["uniforms"], temperature=s["temperature"],
+                                   top_k=s["top_k"], top_p=s["top_p"], min_p=s["min_p"], log_prob=s["log_prob"])
+        return s["tokens"], s["log_prob"]
+    if op == "record":
+        hip.topk_lse_rows(s["logits"], s["values"], s["indices"], lse=s["lse"], temperature=case["temperature"])
+        return s["values"], s["indices"], s["lse"]
+    if op == "linear8":
+        hip.cut_fp8(s["x"], *s["x8"])
+        hip.gemm_fp8(*s["x8"], *s["w8"], s["out"], case["k"], bias=s["bias"])
+        return s["out"]
+    record = dict(teacher_lse=s["t_lse"], temperature=case["temperature"], row_weight=s["weight"])
+    if case["calls"] == "two":
+        hip.distill_loss(s["logits"], s["t_values"], s["t_indices"], s["loss"], stats=s["stats"], **record)
+        hip.distill_grad(s["logits"], s["t_values"], s["t_indices"], s["stats"], s["grad"],
+                         temperature=case["temperature"], row_weight=s["weight"])
+        return s["loss"], s["grad"]
+    if case["calls"] == "fused":
+        hip.distill_loss(s["logits"], s["t_values"], s["t_indices"], s["loss"], dlogits=s["grad"], **record)
+        return s["loss"], s["grad"]
+    hip.distill_loss(s["logits"], s["t_values"], s["t_indices"], s["loss"], **record)
+    return s["loss"]
+
+
+# ---------------------------------------------------------------------------------------------- 64 bits
+def _exact_sample(s, n, v):
+    per_row = {p: np.broadcast_to(s[p].cpu().numpy() if torch.is_tensor(s[p]) else np.asarray(s[p]), (n,))
+               for p in ("temperature", "top_k", "top_p", "min_p")}
+    uniforms = s["uniforms"].cpu().numpy()
+    tokens, log_prob = np.zeros(n, dtype=np.int64), np.zeros(n)
+    for r in range(n):
+        x = s["logits"][r].double().cpu().numpy()
+        temperature, top_p, min_p = (float(per_row[p][r]) for p in ("temperature", "top_p", "min_p"))
+        order = np.lexsort((np.arange(v), -x))
+        if temperature == 0:
+            tokens[r] = order[0]
+            continue
+        if per_row["top_k"][r] > 0:
+            order = order[:int(per_row["top_k"][r])]
+        p = np.exp((x[order] - x[order[0]]) / temperature)
+        cdf = np.cumsum(p)
+        last = int(np.searchsorted(cdf, top_p * cdf[-1], side="left"))
+        order, p = order[:last + 1], p[:last + 1]
+        order, p = order[p >= min_p], p[p >= min_p]
+        by_index = np.argsort(order)
+        order, p = order[by_index], p[by_index]
+        cdf = np.cumsum(p)
+        at = min(int(np.searchsorted(cdf, uniforms[r] * cdf[-1], side="right")), len(order) - 1)
+        tokens[r], log_prob[r] = order[at], np.log(p[at] / cdf[-1])
+    return torch.from_numpy(tokens), torch.from_numpy(log_prob)
+
+
+def exact(case, seed):
+    s = prepare(case, seed)
+    op = case["op"]
+    if op == "linear8":
+        def values(x):
+            rows, k = x.shape
+            out = torch.zeros(rows, k, dtype=torch.float64, device="cuda")
+            for b in range(0, k, BLOCK):
+                part = x[:, b:b + BLOCK].double()
+                big = part.abs().amax(1, keepdim=True)
+                step = torch.exp2(torch.ceil(torch.log2(torch.where(big > 0, big, torch.full_like(big, 448.0)) / 448.0)))
+                out[:, b:b + BLOCK] = (part / step).to(torch.float8_e4m3fn).double() * step
+            return out
+        w = (s["w_codes"].double() * s["w_scale"].double()).flatten(1)[:, :case["k"]]
+        out = values(s["x"]) @ w.t().contiguous()
+        return out if s["bias"] is None else out + s["bias"].double()
+    n, v, t = case["n"], case["v"], case["temperature"]
+    if op == "sample":
+        return _exact_sample(s, n, v)
+    if op == "record":
+        x = s["logits"].cpu().float().numpy()
+        pick = np.stack([np.argsort(-row, kind="stable")[:case["k"]] for row in x])
+        return (torch.from_numpy(np.take_along_axis(x, pick, 1).astype(np.float64)), torch.from_numpy(pick),
+                torch.logsumexp(s["logits"].double() / t, 1))
+    # the divergence over the whole vocabulary, words outside the record as one more word "other"
+    log_p = torch.log_softmax(s["logits"].double() / t, 1)
+    if not case["tail"]:
+        log_q = torch.log_softmax(s["t_values"].double() / t, 1)
+    else:
+        log_q = s["t_values"].double() / t - s["t_lse"].double().view(n, 1)
+    q = log_q.exp()
+    loss = (q * (log_q - log_p.gather(1, s["t_indices"]))).sum(1)
+    p = log_p.exp()
+    sums = q.sum(1)
+    other = torch.zeros(n, 1, dtype=torch.float64, device="cuda")
+    if case["tail"] and case["k"] < v:
+        p_other = p.scatter(1, s["t_indices"], 0.0).sum(1)
+        q_other = (1.0 - sums).clamp(min=0.0)
+        loss = loss + torch.special.xlogy(q_other, q_other) - torch.special.xlogy(q_other, p_other)
+        sums = sums + q_other
+        other = (q_other / p_other).view(n, 1)
+    weight = s["weight"].double()
+    if case["calls"] == "forward":
+        return weight * loss
+    share = torch.zeros_like(p).scatter_(1, s["t_indices"], q)            # the teacher's mass, word by word ...
+    outside = torch.ones_like(p).scatter_(1, s["t_indices"], 0.0)
+    share += outside * p * other                                          # ... "other" shared out as the student does
+    return weight * loss, (p * sums.view(n, 1) - share) * (weight / t).view(n, 1)
