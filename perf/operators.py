@@ -145,7 +145,7 @@ def prepare(case, seed):
     s["weight"] = torch.rand(n, device="cuda", generator=gen) + 0.5
     s["weight"][torch.rand(n, device="cuda", generator=gen) < case["idle"]] = 0.0
     s["loss"] = torch.empty(n, device="cuda")
-    s["stats"] = torch.empty(n, 4, device="cuda")
+    s["stats"] = torch.empty(n, 4, dtype=torch.float64, device="cuda")
     if case["calls"] != "forward":
         s["grad"] = torch.empty(n, v, dtype=s["logits"].dtype, device="cuda")
     return s
