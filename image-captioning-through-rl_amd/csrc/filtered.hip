@@ -1,0 +1,519 @@
+// Rows of logits ranked and filtered: token sampling with temperature, top-k, top-p and min-p, and the k largest
+// entries of a row with its log-normaliser.  One workgroup per row.
+//
+// Both need the same thing, a CUT of the row's order (larger value first, ties by lowest index): the entries that come
+// no later than a certain one.  An entry's place in that order is its composite, (order key of the value) << 32 | ~index,
+// so a cut is one 64-bit number and "kept" is composite >= cut; top-k is the cut after k entries and top-p the cut after
+// the shortest prefix with the wanted mass.  A cut is found from a histogram of the row over 2048 equal value ranges
+// (counts for top-k, masses for top-p), which names the range the cut falls into; the few entries of that range are
+// sorted exactly.  Ranges with more entries than threads (many equal values) are refined by three radix passes over
+// the keys instead.
+//
+// Masses are 64-bit integers, multiples of 2^-S of the row's largest weight with S = 62 - ceil(log2 V) (at most 51):
+// integer sums have no order, so atomics and any split of the row give the same bits, and 2^-45 of the largest weight
+// at V = 131072 is finer than float32 by six orders of magnitude: a draw falls on the side of a border that exact
+// arithmetic gives unless it is that close.
+#include <algorithm>
+#include <math.h>
+
+#include "vocab_row.h"
+
+namespace {
+using namespace icrl;
+
+constexpr int BINS = 2048;
+
+template <int NT>
+struct Shared {
+    u64 hist[BINS];           // histogram; afterwards the list of entries that is sorted
+    u64 part[NT / 64 + 1];    // per-wave sums
+    unsigned key_lo, key_hi;
+    int count, bin, index;
+    u64 above, cut, total;
+    float red[NT / 64];
+    int flag;
+};
+
+__device__ __forceinline__ u64 composite(unsigned key, int index) { return (u64)key << 32 | (unsigned)~index; }
+
+// Weights of one row: e^((x - top) / T) as multiples of 2^-S.
+struct Weights {
+    float top;
+    double per_unit;   // log2(e) / T
+    int S;
+    __device__ __forceinline__ u64 operator()(float x) const {
+        const double t = x == top ? 0.0 : ((double)x - (double)top) * per_unit;
+        if (!(t > -(double)(S + 2))) return 0;
+        const double one = ldexp(exp2_neg(t), S);             // at most 2^51
+        return (u64)(__double_as_longlong(one + 0x1p52) & 0xFFFFFFFFFFFFFll);   // the sum's low 52 bits: `one` to the nearest integer
+    }
+};
+
+template <int NT>
+__device__ __forceinline__ float block_max(float v, float* red) {
+    v = wave_max(v);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    float m = red[0];
+#pragma unroll
+    for (int w = 1; w < NT / 64; ++w) m = fmaxf(m, red[w]);
+    return m;
+}
+
+// Exclusive prefix of v over the workgroup's threads (and the total in sm.total); every thread calls it.
+template <int NT>
+__device__ __forceinline__ u64 block_prefix(u64 v, Shared<NT>& sm) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    u64 inc = v;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const u64 up = __shfl_up(inc, o, 64);
+        if (lane >= o) inc += up;
+    }
+    __syncthreads();
+    if (lane == 63) sm.part[wave] = inc;
+    __syncthreads();
+    u64 before = 0, total = 0;
+#pragma unroll
+    for (int w = 0; w < NT / 64; ++w) {
+        const u64 p = sm.part[w];
+        if (w < wave) before += p;
+        total += p;
+    }
+    sm.total = total;   // every thread writes the same value
+    return before + inc - v;
+}
+
+// Descending sort of one u64 per thread: bitonic, exchanges inside a wave by shuffles, across waves through LDS.
+template <int NT>
+__device__ __forceinline__ u64 block_sort(u64 v, u64* lds) {
+    const int tid = threadIdx.x;
+#pragma unroll
+    for (int size = 2; size <= NT; size <<= 1) {
+        const bool down = (tid & size) == 0 || size == NT;
+#pragma unroll
+        for (int stride = size >> 1; stride > 0; stride >>= 1) {
+            u64 other;
+            if (stride >= 64) {
+                __syncthreads();
+                lds[tid] = v;
+                __syncthreads();
+                other = lds[tid ^ stride];
+            } else {
+                other = __shfl_xor(v, stride, 64);
+            }
+            const bool lower = (tid & stride) == 0;
+            const bool take_larger = lower == down;
+            v = (other > v) == take_larger ? other : v;
+        }
+    }
+    return v;
+}
+
+// Per-wave sums of f(value, index) into sm.part; the total is returned to every thread.
+template <int NT, typename R, typename F>
+__device__ __forceinline__ u64 wave_totals(const R& row, Shared<NT>& sm, F&& f) {
+    u64 mine = 0;
+    row.each([&](float x, int i) { mine += f(x, i); });
+    mine = wave_sum_u64(mine);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) sm.part[threadIdx.x >> 6] = mine;
+    __syncthreads();
+    u64 total = 0;
+#pragma unroll
+    for (int w = 0; w < NT / 64; ++w) total += sm.part[w];
+    return total;
+}
+
+// The index at which the running sum of f in index order first exceeds `target` (< the total that wave_totals has just
+// left per wave).  One wave owns that place; it walks its piece vector by vector.
+template <int NT, typename R, typename F>
+__device__ __forceinline__ int locate(const R& row, Shared<NT>& sm, u64 target, F&& f) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    u64 before = 0;
+    for (int w = 0; w < wave; ++w) before += sm.part[w];
+    if (target >= before && target - before < sm.part[wave]) {
+        u64 left = target - before;
+        bool found = false;
+        for (int i = 0; i < row.vectors && !found; ++i) {
+            const auto p = row.fetch(i);
+            const int at0 = row.first + i * 64 * R::VEC;
+            u64 own = 0;
+            row.vector(p, at0, [&](float x, int at) { own += f(x, at); });
+            u64 inc = own;
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const u64 up = __shfl_up(inc, o, 64);
+                if (lane >= o) inc += up;
+            }
+            const u64 all = __shfl(inc, 63, 64);
+            if (left >= all) {
+                left -= all;
+                continue;
+            }
+            found = true;
+            if (left >= inc - own && left < inc) {
+                u64 run = inc - own;
+                bool done = false;
+                row.vector(p, at0, [&](float x, int at) {
+                    run += f(x, at);
+                    if (!done && run > left) { sm.index = at; done = true; }
+                });
+            }
+        }
+    }
+    __syncthreads();
+    return sm.index;
+}
+
+// Where the running sum of sm.hist (bin 0 first) reaches `need` (which need_of makes from the total): bin in sm.bin, the
+// sum of the bins before it in sm.above.  Returns need.
+template <int NT, typename G>
+__device__ __forceinline__ u64 find_bin(Shared<NT>& sm, G&& need_of) {
+    constexpr int PER = BINS / NT;
+    u64 own[PER], sum = 0;
+#pragma unroll
+    for (int b = 0; b < PER; ++b) {
+        own[b] = sm.hist[threadIdx.x * PER + b];
+        sum += own[b];
+    }
+    u64 run = block_prefix<NT>(sum, sm);
+    const u64 need = need_of(sm.total);
+    if (run < need && run + sum >= need) {
+        bool done = false;
+#pragma unroll
+        for (int b = 0; b < PER; ++b) {
+            if (!done && run + own[b] >= need) { sm.bin = threadIdx.x * PER + b; sm.above = run; done = true; }
+            run += own[b];
+        }
+    }
+    __syncthreads();
+    return need;
+}
+
+template <int NT>
+__device__ __forceinline__ void clear_hist(Shared<NT>& sm) {
+    __syncthreads();
+    for (int b = threadIdx.x; b < BINS; b += NT) sm.hist[b] = 0;
+    __syncthreads();
+}
+
+// The cut after the shortest prefix (in the row's order, among the entries with composite >= `from`) whose amounts -
+// MASS: weights, else 1 each - reach need_of(total).  width: the value range that the first histogram spreads over its
+// bins, counted from the top; any positive width gives the same cut, a good one makes the second step short.
+template <bool MASS, int NT, typename R, typename G>
+__device__ __forceinline__ u64 find_cut(const R& row, Shared<NT>& sm, u64 from, const Weights& weight, float width, G&& need_of) {
+    const unsigned from_key = (unsigned)(from >> 32);
+    const unsigned from_index = ~(unsigned)from;
+    auto kept = [&](unsigned key, int i) { return key > from_key || (key == from_key && (unsigned)i <= from_index); };
+    auto amount = [&](float x) { return MASS ? weight(x) : (u64)1; };
+    const float per = (float)BINS / width, top = weight.top;
+    auto bin = [&](float x) {   // monotone in the row's order; what is far below the top, NaN included, is the last bin
+        const float at = (top - x) * per;
+        return at < (float)(BINS - 1) ? (int)at : BINS - 1;
+    };
+    clear_hist<NT>(sm);
+    if (threadIdx.x == 0) { sm.count = 0; sm.key_lo = ~0u; sm.key_hi = 0; }
+    u64 rest = 0;   // the last bin, which may hold most of the row, is summed in registers
+    row.each([&](float x, int i) {
+        if (kept(order_key(x), i)) {
+            const u64 a = amount(x);
+            const int b = bin(x);
+            if (b == BINS - 1) rest += a;
+            else if (a) atomicAdd(&sm.hist[b], a);
+        }
+    });
+    rest = wave_sum_u64(rest);
+    if ((threadIdx.x & 63) == 0 && rest) atomicAdd(&sm.hist[BINS - 1], rest);
+    __syncthreads();
+    u64 need = find_bin<NT>(sm, need_of);
+    const int b0 = sm.bin;
+    need -= sm.above;
+    __syncthreads();   // the histogram's place now takes the entries of that bin
+    row.each([&](float x, int i) {
+        const unsigned key = order_key(x);
+        if (kept(key, i) && bin(x) == b0) {
+            const int at = atomicAdd(&sm.count, 1);
+            if (at < NT) sm.hist[at] = composite(key, i);
+        }
+    });
+    __syncthreads();
+    const int members = sm.count;
+    if (members <= NT) {
+        u64 c = (int)threadIdx.x < members ? sm.hist[threadIdx.x] : 0;
+        c = block_sort<NT>(c, sm.hist);
+        u64 a = 0;
+        if (c != 0) {
+            const unsigned key = (unsigned)(c >> 32);
+            const float x = __uint_as_float(key ^ ((key >> 31) ? 0x80000000u : 0xFFFFFFFFu));
+            a = amount(x);
+        }
+        const u64 before = block_prefix<NT>(a, sm);
+        if (before < need && before + a >= need) sm.cut = c;
+        __syncthreads();
+        return sm.cut;
+    }
+    // many entries in one range: radix over the keys that occur in it, 11 bits a pass
+    unsigned lo = ~0u, hi = 0;
+    row.each([&](float x, int i) {
+        const unsigned key = order_key(x);
+        if (kept(key, i) && bin(x) == b0) { lo = min(lo, key); hi = max(hi, key); }
+    });
+    atomicMin(&sm.key_lo, lo);
+    atomicMax(&sm.key_hi, hi);
+    __syncthreads();
+    lo = sm.key_lo;
+    hi = sm.key_hi;
+    while (lo < hi) {
+        const int bits = 32 - __clz((int)(hi - lo)), shift = bits > 11 ? bits - 11 : 0;
+        clear_hist<NT>(sm);
+        row.each([&](float x, int i) {
+            const unsigned key = order_key(x);
+            if (key >= lo && key <= hi && kept(key, i) && bin(x) == b0) {
+                const u64 a = amount(x);
+                if (a) atomicAdd(&sm.hist[(hi - key) >> shift], a);
+            }
+        });
+        __syncthreads();
+        const u64 want = need;
+        find_bin<NT>(sm, [&](u64) { return want; });
+        need -= sm.above;
+        const unsigned upper = hi - ((unsigned)sm.bin << shift);
+        const unsigned span = (1u << shift) - 1u;
+        lo = upper - lo > span ? upper - span : lo;
+        hi = upper;
+        __syncthreads();
+    }
+    // the entries with this key, in index order, until they reach what is left
+    const float x = __uint_as_float(lo ^ ((lo >> 31) ? 0x80000000u : 0xFFFFFFFFu));
+    const u64 each = amount(x);
+    auto tie = [&](float y, int i) { const unsigned key = order_key(y); return (u64)(key == lo && kept(key, i)); };
+    wave_totals<NT>(row, sm, tie);
+    const int last = locate<NT>(row, sm, (need + each - 1) / each - 1, tie);
+    __syncthreads();
+    return composite(lo, last);
+}
+
+// ---------------------------------------------------------------------------------------------- sampling
+struct Setting {   // one filter setting: a value for each row, or one for all of them
+    const float* rows;
+    double all;
+    __device__ __forceinline__ double at(int r) const { return rows ? (double)rows[r] : all; }
+};
+
+template <typename T, int NT, int PLACE>
+__global__ __launch_bounds__(NT) void sample_filtered_kernel(const T* __restrict__ logits, int64_t ld, int V, int S,
+                                                             const double* __restrict__ uniforms, Setting temperature,
+                                                             const int* __restrict__ top_k_rows, int top_k_all,
+                                                             Setting top_p_in, Setting min_p_in,
+                                                             int64_t* __restrict__ tokens, int64_t token_stride,
+                                                             float* __restrict__ log_prob, int64_t lp_stride) {
+    __shared__ Shared<NT> sm;
+    const int r = blockIdx.x, tid = threadIdx.x;
+    Row<T, NT, PLACE, true> row;
+    extern __shared__ __attribute__((aligned(16))) unsigned char staged[];
+    row.open(logits + (int64_t)r * ld, V, staged);
+    const double temp = temperature.at(r), top_p = top_p_in.at(r), min_p = min_p_in.at(r), u = uniforms[r];
+    const int top_k = top_k_rows ? top_k_rows[r] : top_k_all;
+    if (tid == 0) sm.flag = 0;
+    float best = -INFINITY;
+    bool nan = false;
+    row.each([&](float x, int i) {
+        best = fmaxf(best, x);                       // fmaxf passes over NaN
+        nan |= x != x && i < V;
+    });
+    best = block_max<NT>(best, sm.red);
+    if (nan) sm.flag = 1;
+    __syncthreads();
+    const bool fine = temp >= 0.0 && temp < INFINITY && top_k >= 0 && top_p >= 0.0 && top_p <= 1.0 && min_p >= 0.0 &&
+                      min_p <= 1.0 && u == u;
+    if (!fine || sm.flag || best == -INFINITY) {
+        if (tid == 0) {
+            tokens[r * token_stride] = -1;
+            if (log_prob) log_prob[r * lp_stride] = NAN;
+        }
+        return;
+    }
+    // with an entry of +inf only the entries of +inf have weight (all the same)
+    const unsigned least = best == INFINITY ? kKeyPlusInf : kKeyFinite;
+    u64 cut = (u64)least << 32;
+    if (temp == 0.0 || top_k == 1 || top_p == 0.0) {   // the first largest entry
+        wave_totals<NT>(row, sm, [&](float x, int) { return (u64)(x == best); });
+        const int at = locate<NT>(row, sm, 0, [&](float x, int) { return (u64)(x == best); });
+        if (tid == 0) {
+            tokens[r * token_stride] = at;
+            if (log_prob) log_prob[r * lp_stride] = 0.f;
+        }
+        return;
+    }
+    const Weights weight{best, 1.4426950408889634074 / temp, S};
+    const float reach = (float)(S * 0.6931471805599453 * temp);   // entries further below the top weigh nothing
+    if (top_k > 0 && top_k < V) {
+        const u64 k = (u64)top_k;
+        const u64 c = find_cut<false, NT>(row, sm, cut, weight, fmaxf(reach, 1e-30f),
+                                          [&](u64 total) { return k < total ? k : total; });
+        cut = c > cut ? c : cut;
+    }
+    if (top_p < 1.0)
+        cut = find_cut<true, NT>(row, sm, cut, weight, fmaxf(reach, 1e-30f), [&](u64 total) {
+            const double w = ceil(top_p * (double)total);
+            const u64 want = w < 1.0 ? 1 : (u64)w;
+            return want < total ? want : total;
+        });
+    const unsigned cut_key = (unsigned)(cut >> 32);
+    const unsigned cut_index = ~(unsigned)cut;
+    const double floor_z = min_p > 0.0 ? log(min_p) * temp : -INFINITY;   // w >= min_p as x - top >= T log(min_p)
+    auto mass = [&](float x, int i) -> u64 {
+        const unsigned key = order_key(x);
+        if (!(key > cut_key || (key == cut_key && (unsigned)i <= cut_index))) return 0;
+        if (x != best && (double)x - (double)best < floor_z) return 0;
+        return weight(x);
+    };
+    const u64 total = wave_totals<NT>(row, sm, mass);
+    const double want = u * (double)total;
+    u64 target = want > 0.0 ? (u64)fmin(want, 0x1p63) : 0;
+    if (target >= total) target = total - 1;
+    const int token = locate<NT>(row, sm, target, mass);
+    if (tid == 0) {
+        tokens[r * token_stride] = token;
+        if (log_prob) {
+            const float x = Elem<T>::value(__builtin_bit_cast(typename Elem<T>::Raw, row.src[token]));
+            const double z = x == best ? 0.0 : ((double)x - (double)best) / temp;
+            log_prob[r * lp_stride] = (float)(z - log(ldexp((double)total, -S)));
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------- top-k and log-normaliser
+template <typename T, int NT, int PLACE>
+__global__ __launch_bounds__(NT) void topk_lse_kernel(const T* __restrict__ logits, int64_t ld, int V, int k, double per_t,
+                                                      float* __restrict__ values, int64_t* __restrict__ indices,
+                                                      float* __restrict__ lse) {
+    __shared__ Shared<NT> sm;
+    __shared__ double sums[NT / 64];
+    const int r = blockIdx.x, tid = threadIdx.x;
+    Row<T, NT, PLACE, true> row;
+    extern __shared__ __attribute__((aligned(16))) unsigned char staged[];
+    row.open(logits + (int64_t)r * ld, V, staged);
+    float best = -INFINITY, low = INFINITY;
+    bool nan = false;
+    if (tid == 0) sm.flag = 0;
+    row.each([&](float x, int i) {
+        best = fmaxf(best, x);
+        nan |= x != x && i < V;
+    });
+    low = best;   // the thread's own largest: the k-th largest of the row is no lower than the lowest of k threads'
+    best = block_max<NT>(best, sm.red);
+    if (nan) sm.flag = 1;
+    if (lse) {
+        double s = 0.0;
+        if (best > -INFINITY && best < INFINITY) {
+            const float c = (float)(per_t * 1.4426950408889634074);
+            float part = 0.f;
+            row.each([&](float x, int) { if (x == x) part += __builtin_amdgcn_exp2f((x - best) * c); });
+            s = part;
+        }
+        s = wave_sum_d(s);
+        __syncthreads();
+        if ((tid & 63) == 0) sums[tid >> 6] = s;
+        __syncthreads();
+        if (tid == 0) {
+            s = 0.0;
+            for (int w = 0; w < NT / 64; ++w) s += sums[w];
+            const bool some = best > -INFINITY && best < INFINITY;
+            lse[r] = sm.flag ? NAN : some ? (float)((double)best * per_t + log(s)) : best;
+        }
+    }
+    const float lowest = -block_max<NT>(-low, sm.red);
+    const float width = lowest > -INFINITY && best < INFINITY ? fmaxf((best - lowest) * 1.001f, 1e-30f) : 64.f;
+    const Weights weight{best, 0.0, 0};
+    const u64 want = (u64)k;
+    const u64 cut = find_cut<false, NT>(row, sm, (u64)kKeyNan << 32, weight, width, [&](u64) { return want; });
+    __syncthreads();
+    if (tid == 0) sm.count = 0;
+    __syncthreads();
+    row.each([&](float x, int i) {
+        const u64 c = composite(order_key(x), i);
+        if (c >= cut) sm.hist[atomicAdd(&sm.count, 1)] = c;   // exactly k entries, k <= NT
+    });
+    __syncthreads();
+    u64 c = tid < k ? sm.hist[tid] : 0;
+    c = block_sort<NT>(c, sm.hist);
+    if (tid < k) {
+        const unsigned key = (unsigned)(c >> 32);
+        const int i = (int)~(unsigned)c;
+        values[(int64_t)r * k + tid] = __uint_as_float(key ^ ((key >> 31) ? 0x80000000u : 0xFFFFFFFFu));
+        indices[(int64_t)r * k + tid] = i;
+    }
+}
+
+constexpr int MAX_K = 1024, MAX_V = 1 << 22;
+
+// Workgroup size, and whether the row is staged in LDS, for rows of V entries of which `list` are to be ranked.
+#define ICRL_ROW_DISPATCH(T, V, list, CALL)                                                                       \
+    do {                                                                                                          \
+        constexpr int vec_ = icrl::Elem<T>::VEC;                                                                  \
+        if ((V) <= 256 * 4 * vec_ && (list) <= 256) { CALL(T, 256, IN_LDS); }                                     \
+        else if ((V) <= 512 * 8 * vec_ && (list) <= 512) { CALL(T, 512, IN_LDS); }                                \
+        else { CALL(T, 1024, IN_MEMORY); }                                                                        \
+    } while (0)
+template <typename T, int NT, int PLACE>
+size_t staged_bytes(int V) {
+    if constexpr (PLACE == IN_LDS) return (size_t)16 * Row<T, NT, PLACE, true>::lds_vectors(V);
+    else return 0;
+}
+}  // namespace
+
+extern "C" int icrl_sample_tokens_filtered(const void* logits, int dtype, int64_t ld_logits, int N, int V,
+                                           const double* uniforms, const float* temperature_rows, double temperature,
+                                           const int32_t* top_k_rows, int top_k, const float* top_p_rows, double top_p,
+                                           const float* min_p_rows, double min_p, int64_t* tokens_out,
+                                           int64_t token_stride, float* log_prob, int64_t log_prob_stride,
+                                           icrl_stream_t stream) {
+    ICRL_REQUIRE(logits && uniforms && tokens_out && N > 0 && V > 0, "icrl_sample_tokens_filtered: null pointer or empty shape");
+    ICRL_REQUIRE(ld_logits >= V, "icrl_sample_tokens_filtered: ld_logits < V");
+    ICRL_REQUIRE(V <= MAX_V, "icrl_sample_tokens_filtered: vocabulary %d exceeds %d entries", V, MAX_V);
+    ICRL_REQUIRE(temperature_rows || (temperature >= 0.0 && isfinite(temperature)), "icrl_sample_tokens_filtered: temperature must be finite and not negative");
+    ICRL_REQUIRE(top_k_rows || top_k >= 0, "icrl_sample_tokens_filtered: top_k must not be negative (0: off)");
+    ICRL_REQUIRE(top_p_rows || (top_p >= 0.0 && top_p <= 1.0), "icrl_sample_tokens_filtered: top_p must be in [0, 1]");
+    ICRL_REQUIRE(min_p_rows || (min_p >= 0.0 && min_p <= 1.0), "icrl_sample_tokens_filtered: min_p must be in [0, 1]");
+    int bits = 0;
+    while ((1 << bits) < V) ++bits;
+    const int S = std::min(51, 62 - bits);
+    const Setting t{temperature_rows, temperature}, p{top_p_rows, top_p}, q{min_p_rows, min_p};
+#define ICRL_CALL(T, NT, PLACE)                                                                                           \
+    hipLaunchKernelGGL((sample_filtered_kernel<T, NT, PLACE>), dim3(N), dim3(NT), (staged_bytes<T, NT, PLACE>(V)), icrl::as_stream(stream),             \
+                       static_cast<const T*>(logits), ld_logits, V, S, uniforms, t, top_k_rows, top_k, p, q, tokens_out, \
+                       token_stride, log_prob, log_prob_stride)
+    switch (dtype) {
+        case ICRL_F32: ICRL_ROW_DISPATCH(float, V, 0, ICRL_CALL); break;
+        case ICRL_BF16: ICRL_ROW_DISPATCH(__bf16, V, 0, ICRL_CALL); break;
+        case ICRL_F16: ICRL_ROW_DISPATCH(_Float16, V, 0, ICRL_CALL); break;
+        default: icrl::set_error("icrl_sample_tokens_filtered: unknown dtype %d", dtype); return ICRL_ERR_ARG;
+    }
+#undef ICRL_CALL
+    ICRL_LAUNCH_CHECK();
+    return ICRL_OK;
+}
+
+extern "C" int icrl_topk_lse_rows(const void* logits, int dtype, int64_t ld_logits, int N, int V, int k, double temperature,
+                                  float* values, int64_t* indices, float* lse, icrl_stream_t stream) {
+    ICRL_REQUIRE(logits && values && indices && N > 0 && V > 0, "icrl_topk_lse_rows: null pointer or empty shape");
+    ICRL_REQUIRE(ld_logits >= V, "icrl_topk_lse_rows: ld_logits < V");
+    ICRL_REQUIRE(V <= MAX_V, "icrl_topk_lse_rows: vocabulary %d exceeds %d entries", V, MAX_V);
+    ICRL_REQUIRE(k >= 1 && k <= V && k <= MAX_K, "icrl_topk_lse_rows: k must be in [1, min(%d, V)] (got %d)", MAX_K, k);
+    ICRL_REQUIRE(temperature > 0.0 && isfinite(temperature), "icrl_topk_lse_rows: temperature must be positive and finite");
+#define ICRL_CALL(T, NT, PLACE)                                                                                     \
+    hipLaunchKernelGGL((topk_lse_kernel<T, NT, PLACE>), dim3(N), dim3(NT), (staged_bytes<T, NT, PLACE>(V)), icrl::as_stream(stream),              \
+                       static_cast<const T*>(logits), ld_logits, V, k, 1.0 / temperature, values, indices, lse)
+    switch (dtype) {
+        case ICRL_F32: ICRL_ROW_DISPATCH(float, V, k, ICRL_CALL); break;
+        case ICRL_BF16: ICRL_ROW_DISPATCH(__bf16, V, k, ICRL_CALL); break;
+        case ICRL_F16: ICRL_ROW_DISPATCH(_Float16, V, k, ICRL_CALL); break;
+        default: icrl::set_error("icrl_topk_lse_rows: unknown dtype %d", dtype); return ICRL_ERR_ARG;
+    }
+#undef ICRL_CALL
+    ICRL_LAUNCH_CHECK();
+    return ICRL_OK;
+}

@@ -1,0 +1,334 @@
+// Products of 8-bit operands (e4m3) with one power-of-two scale for each row and block of 128 along k, in two ways:
+//
+// 16-bit outputs run on the scaled matrix instruction v_mfma_scale_f32_32x32x64_f8f6f4, which multiplies each lane's 32
+// products by the two scales (bytes holding the exponent + 127) as it adds them up: a scale costs no instruction.  It
+// does not keep every bit: of each 8 products in a row it drops what lies more than 13 binary places below the largest
+// one's 2^(exponent a + exponent b) (found with sums of one large and one small product), which leaves sums of random
+// terms off by 8e-6 of their size - far below a 16-bit output's rounding, but not below float32's.
+//
+// float32 outputs therefore turn the codes, scale included, into bf16 (v_cvt_scalef32_pk_bf16_fp8: exact, four
+// significant bits of eight) and multiply those at half the rate, with exact products and float32 sums (3e-8).
+//
+// Operands are cut once by icrl_cut_fp8 into the instruction's fragment order (rows and k padded with zeros), like
+// icrl_cut_f16x2's: rows in blocks of 32, k in blocks of 64; a block is 2048 bytes, lane l = row % 32 + 32 (k % 64 / 32)
+// holding 32 codes as two 16-byte halves, half h of all lanes before half h + 1.  Any 1 KB of it is one wave's 16-byte
+// load, into registers or straight into LDS, and a fragment's reads from LDS have no bank conflicts.  Scales: one byte
+// per row and block of 128; four blocks of a row to a 32-bit word, words of a 32-row block side by side.
+#include <algorithm>
+#include <type_traits>
+
+#include "vocab_row.h"
+
+namespace {
+using namespace icrl;
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+constexpr int BLOCK = 128;
+inline int blocks128(int K) { return (K + BLOCK - 1) / BLOCK; }
+inline int scale_words(int K) { return (blocks128(K) + 3) / 4; }   // 32-bit words of scales per row
+
+// Eight lanes cut one row's block of 128: 16 entries a lane, which are one 16-byte half of the fragment's lane.
+template <typename T>
+__global__ __launch_bounds__(256) void cut_kernel(const T* __restrict__ x, int64_t ld, int rows, int K, int nblocks, int words,
+                                                  unsigned char* __restrict__ pieces, unsigned char* __restrict__ scales) {
+    const int lane8 = threadIdx.x & 7;
+    const int64_t unit = (int64_t)blockIdx.x * 32 + (threadIdx.x >> 3);   // (row, group of four blocks' block)
+    const int padded = words * 4;
+    const int row = (int)(unit / padded), b = (int)(unit % padded);
+    if (row >= (rows + 31) / 32 * 32) return;
+    const int k0 = b * BLOCK + lane8 * 16;
+    float v[16];
+    unsigned top = 0;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v[j] = 0.f;
+    if (row < rows && k0 < K) {
+        const T* src = x + (int64_t)row * ld + k0;
+        if (k0 + 16 <= K) {
+            constexpr int VEC = Elem<T>::VEC;
+#pragma unroll
+            for (int q = 0; q < 16 / VEC; ++q) {
+                typename Elem<T>::Raw raw[VEC];
+                __builtin_memcpy(raw, src + q * VEC, 16);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) v[q * VEC + j] = Elem<T>::value(raw[j]);
+            }
+        } else {
+            for (int j = 0; j < 16; ++j)
+                if (k0 + j < K) v[j] = (float)src[j];
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 16; ++j) top = max(top, __float_as_uint(v[j]) & 0x7FFFFFFFu);
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) top = max(top, (unsigned)__shfl_xor((int)top, o, 64));
+    // the smallest power of two 2^e with top <= 448 2^e (448 = 1.75 2^8 is the type's largest value)
+    int e = (int)(top >> 23) - 127 - 8 + ((top & 0x7FFFFFu) > 0x600000u ? 1 : 0);
+    e = top == 0 ? 0 : max(e, -127);
+    const bool finite = top < 0x7F800000u;   // a block with an infinity or a NaN: the scale is NaN
+    if (lane8 == 0) scales[(((int64_t)(row >> 5) * words + (b >> 2)) * 32 + (row & 31)) * 4 + (b & 3)] = finite ? (unsigned char)(e + 127) : 255;
+    if (b >= nblocks) return;
+    const float inv = finite ? ldexpf(1.f, -e) : 0.f;
+    i32x4 out;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {   // exact scaling, then one rounding to nearest even
+        int w = 0;
+        w = __builtin_amdgcn_cvt_pk_fp8_f32(finite ? v[4 * q] * inv : 0.f, finite ? v[4 * q + 1] * inv : 0.f, w, false);
+        w = __builtin_amdgcn_cvt_pk_fp8_f32(finite ? v[4 * q + 2] * inv : 0.f, finite ? v[4 * q + 3] * inv : 0.f, w, true);
+        out[q] = w;
+    }
+    const int kb = 2 * b + (lane8 >> 2), half = lane8 & 1, group = lane8 >> 1 & 1;
+    unsigned char* dst = pieces + ((((int64_t)(row >> 5) * (2 * nblocks) + kb) * 2 + half) * 64 + (row & 31) + 32 * group) * 16;
+    *reinterpret_cast<i32x4*>(dst) = out;
+}
+
+template <typename T>
+__device__ __forceinline__ void store_out(T* p, float x) { *p = (T)x; }
+
+struct Operand {
+    const unsigned char* pieces;
+    const unsigned* scales;
+    int row_blocks;
+};
+
+__device__ __forceinline__ i32x8 join(i32x4 a, i32x4 b) {
+    return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+// A lane's 32 codes of a block of 64, as the multiplication takes them, with their scale (its byte in the low 8 bits).
+struct ScaledFragment {
+    i32x8 codes;
+    unsigned scale;
+    ScaledFragment() = default;
+    __device__ __forceinline__ ScaledFragment(i32x4 lo, i32x4 hi, unsigned s) : codes(join(lo, hi)), scale(s) {}
+};
+__device__ __forceinline__ void multiply(const ScaledFragment& a, const ScaledFragment& b, f32x16& acc) {
+    acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a.codes, b.codes, acc, 0, 0, 0, (int)a.scale, 0, (int)b.scale);
+}
+
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+struct ExactFragment {
+    bf16x8 part[4];   // 8 codes each: which k they are does not matter as long as both operands agree
+    ExactFragment() = default;
+    __device__ __forceinline__ ExactFragment(i32x4 lo, i32x4 hi, unsigned s) {
+        const unsigned byte = s & 255u;
+        const float scale = __uint_as_float(byte == 255u ? 0x7FC00000u : byte << 23);
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+                const unsigned codes = (unsigned)(q < 2 ? lo[2 * q + w] : hi[2 * q - 4 + w]);
+                const bf16x2 l = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, scale, false);
+                const bf16x2 h = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, scale, true);
+                part[q][4 * w] = l[0]; part[q][4 * w + 1] = l[1];
+                part[q][4 * w + 2] = h[0]; part[q][4 * w + 3] = h[1];
+            }
+    }
+};
+__device__ __forceinline__ void multiply(const ExactFragment& a, const ExactFragment& b, f32x16& acc) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.part[q], b.part[q], acc, 0, 0, 0);
+}
+template <typename T>
+using Fragment = std::conditional_t<sizeof(T) == 4, ExactFragment, ScaledFragment>;
+
+// ---- few rows: one 32 x 32 tile of the output per workgroup, k cut over its waves, fragments straight from memory
+template <typename T, int WAVES>
+__global__ __launch_bounds__(WAVES * 64) void gemm_fp8_rows(Operand a, Operand b, T* __restrict__ out, int64_t ldo, int M, int N,
+                                                            int nblocks, int words, const float* __restrict__ bias) {
+    __shared__ float part[WAVES][16][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int rb_n = blockIdx.x, rb_m = blockIdx.y;
+    const i32x4* pa = reinterpret_cast<const i32x4*>(a.pieces) + (int64_t)rb_m * nblocks * 256 + lane;
+    const i32x4* pb = reinterpret_cast<const i32x4*>(b.pieces) + (int64_t)rb_n * nblocks * 256 + lane;
+    const unsigned* sa = a.scales + (int64_t)rb_m * words * 32 + (lane & 31);
+    const unsigned* sb = b.scales + (int64_t)rb_n * words * 32 + (lane & 31);
+    f32x16 acc = {};
+    for (int blk = wave; blk < nblocks; blk += WAVES) {
+        i32x4 fa[4], fb[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) { fb[q] = pb[(int64_t)blk * 256 + q * 64]; fa[q] = pa[(int64_t)blk * 256 + q * 64]; }
+        const unsigned ea = sa[(blk >> 2) * 32] >> (8 * (blk & 3)), eb = sb[(blk >> 2) * 32] >> (8 * (blk & 3));
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+            multiply(Fragment<T>(fa[2 * q], fa[2 * q + 1], ea), Fragment<T>(fb[2 * q], fb[2 * q + 1], eb), acc);
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) part[wave][i][lane] = acc[i];
+    __syncthreads();
+    for (int e = threadIdx.x; e < 1024; e += WAVES * 64) {
+        const int i = e >> 6, l = e & 63;
+        const int m = rb_m * 32 + 8 * (i >> 2) + 4 * (l >> 5) + (i & 3), n = rb_n * 32 + (l & 31);
+        float s = 0.f;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) s += part[w][i][l];
+        if (m < M && n < N) store_out(out + (int64_t)m * ldo + n, s + (bias ? bias[n] : 0.f));
+    }
+}
+
+// ---- tiles of (64 WM) x (64 WN) per workgroup of 2 x 2 waves, operands staged through LDS a block of 128 at a time, the
+// next block's copy in flight (straight into LDS) while the current one is multiplied
+template <typename T, int WM, int WN>
+__global__ __launch_bounds__(256) void gemm_fp8_tiles(Operand a, Operand b, T* __restrict__ out, int64_t ldo, int M, int N,
+                                                      int nblocks, int words, const float* __restrict__ bias, int tiles_m,
+                                                      int tiles_n) {
+    constexpr int RA = 2 * WM, RB = 2 * WN;                 // 32-row blocks per tile
+    constexpr int STAGE = (RA + RB) * 4096;                 // bytes of one block of 128
+    __shared__ __attribute__((aligned(16))) unsigned char lds[2 * STAGE];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave >> 1, wn = wave & 1;
+    // workgroups go round the 8 XCDs: give each XCD a contiguous run of tiles, in bands of 8 tile rows, so that what
+    // its L2 holds is shared by the tiles it works on
+    const int total = tiles_m * tiles_n;
+    int t = blockIdx.x;
+    {
+        const int per = total / 8, extra = total % 8, xcd = t % 8, at = t / 8;
+        t = xcd * per + min(xcd, extra) + at;
+    }
+    const int band = t / (8 * tiles_n), in_band = t % (8 * tiles_n), rows_in_band = min(8, tiles_m - 8 * band);
+    const int tm = 8 * band + in_band % rows_in_band, tn = in_band / rows_in_band;
+    auto stage = [&](int blk, int buf) {
+        unsigned char* base = lds + buf * STAGE;
+#pragma unroll
+        for (int q = 0; q < RA + RB; ++q) {
+            // one 4 KB piece (a row block's block of 128) per step: each wave copies 1 KB of it
+            const bool is_a = q < RA;
+            const Operand& o = is_a ? a : b;
+            const int rb = min(is_a ? tm * RA + q : tn * RB + (q - RA), o.row_blocks - 1);   // past the end: any rows, never stored
+            const unsigned char* src = o.pieces + ((int64_t)rb * nblocks + blk) * 4096 + wave * 1024 + lane * 16;
+            unsigned char* dst = base + q * 4096 + wave * 1024;
+            __builtin_amdgcn_global_load_lds(reinterpret_cast<const __attribute__((address_space(1))) unsigned*>(reinterpret_cast<uintptr_t>(src)),
+                                             (__attribute__((address_space(3))) unsigned*)dst, 16, 0, 0);
+        }
+    };
+    f32x16 acc[WM][WN] = {};
+    const unsigned* sa[WM];
+    const unsigned* sb[WN];
+#pragma unroll
+    for (int i = 0; i < WM; ++i) sa[i] = a.scales + (int64_t)min(tm * RA + wm * WM + i, a.row_blocks - 1) * words * 32 + (lane & 31);
+#pragma unroll
+    for (int i = 0; i < WN; ++i) sb[i] = b.scales + (int64_t)min(tn * RB + wn * WN + i, b.row_blocks - 1) * words * 32 + (lane & 31);
+    unsigned ea[WM], eb[WN];
+    stage(0, 0);
+    for (int blk = 0; blk < nblocks; ++blk) {
+        if ((blk & 3) == 0) {
+#pragma unroll
+            for (int i = 0; i < WM; ++i) ea[i] = sa[i][(blk >> 2) * 32];
+#pragma unroll
+            for (int i = 0; i < WN; ++i) eb[i] = sb[i][(blk >> 2) * 32];
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // each wave waits for its own part of this block's copy,
+        __syncthreads();                                   // then for the others'; the other buffer is free by now
+        if (blk + 1 < nblocks) stage(blk + 1, (blk + 1) & 1);
+        const unsigned char* base = lds + (blk & 1) * STAGE + lane * 16;
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+            auto fragment = [&](int rb, unsigned scale) {
+                const unsigned char* p = base + rb * 4096 + kk * 2048;
+                return Fragment<T>(*reinterpret_cast<const i32x4*>(p), *reinterpret_cast<const i32x4*>(p + 1024), scale);
+            };
+            Fragment<T> fb[WN];
+#pragma unroll
+            for (int j = 0; j < WN; ++j) fb[j] = fragment(RA + wn * WN + j, eb[j]);
+#pragma unroll
+            for (int i = 0; i < WM; ++i) {
+                const Fragment<T> fa = fragment(wm * WM + i, ea[i]);
+#pragma unroll
+                for (int j = 0; j < WN; ++j) multiply(fa, fb[j], acc[i][j]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < WM; ++i) ea[i] >>= 8;
+#pragma unroll
+        for (int i = 0; i < WN; ++i) eb[i] >>= 8;
+    }
+#pragma unroll
+    for (int j = 0; j < WN; ++j) {
+        const int n = (tn * RB + wn * WN + j) * 32 + (lane & 31);
+        const float add = bias && n < N ? bias[n] : 0.f;
+#pragma unroll
+        for (int i = 0; i < WM; ++i) {
+            const int m0 = (tm * RA + wm * WM + i) * 32 + 4 * (lane >> 5);
+#pragma unroll
+            for (int q = 0; q < 16; ++q) {
+                const int m = m0 + 8 * (q >> 2) + (q & 3);
+                if (m < M && n < N) store_out(out + (int64_t)m * ldo + n, acc[i][j][q] + add);
+            }
+        }
+    }
+}
+}  // namespace
+
+extern "C" int64_t icrl_fp8_piece_bytes(int rows, int K) {
+    return rows > 0 && K > 0 ? (int64_t)((rows + 31) / 32 * 32) * blocks128(K) * BLOCK : 0;
+}
+extern "C" int64_t icrl_fp8_scale_bytes(int rows, int K) {
+    return rows > 0 && K > 0 ? (int64_t)((rows + 31) / 32 * 32) * scale_words(K) * 4 : 0;
+}
+
+extern "C" int icrl_cut_fp8(const void* x, int dtype, int64_t ld, int rows, int K, void* pieces, void* scales, icrl_stream_t stream) {
+    ICRL_REQUIRE(x && pieces && scales && rows > 0 && K > 0, "icrl_cut_fp8: null pointer or empty shape");
+    ICRL_REQUIRE(ld >= K, "icrl_cut_fp8: row stride < K");
+    ICRL_REQUIRE(reinterpret_cast<uintptr_t>(pieces) % 16 == 0 && reinterpret_cast<uintptr_t>(scales) % 4 == 0,
+                 "icrl_cut_fp8: pieces must be 16-byte aligned, scales 4-byte");
+    const int words = scale_words(K), nb = blocks128(K);
+    const int64_t units = (int64_t)((rows + 31) / 32 * 32) * words * 4, grid = (units + 31) / 32;
+    ICRL_REQUIRE(grid <= 0x7FFFFFFF, "icrl_cut_fp8: operand too large");
+#define ICRL_CALL(T)                                                                                              \
+    hipLaunchKernelGGL((cut_kernel<T>), dim3((unsigned)grid), dim3(256), 0, icrl::as_stream(stream),              \
+                       static_cast<const T*>(x), ld, rows, K, nb, words, static_cast<unsigned char*>(pieces),     \
+                       static_cast<unsigned char*>(scales))
+    switch (dtype) {
+        case ICRL_F32: ICRL_CALL(float); break;
+        case ICRL_BF16: ICRL_CALL(__bf16); break;
+        case ICRL_F16: ICRL_CALL(_Float16); break;
+        default: icrl::set_error("icrl_cut_fp8: unknown dtype %d", dtype); return ICRL_ERR_ARG;
+    }
+#undef ICRL_CALL
+    ICRL_LAUNCH_CHECK();
+    return ICRL_OK;
+}
+
+namespace {
+template <typename T>
+void launch_gemm(const Operand& a, const Operand& b, T* out, int64_t ldo, int M, int N, int K, const float* bias, hipStream_t st) {
+    const int nb = blocks128(K), words = scale_words(K);
+    if (M <= 64) {
+        hipLaunchKernelGGL((gemm_fp8_rows<T, 4>), dim3(b.row_blocks, a.row_blocks), dim3(256), 0, st, a, b, out, ldo, M, N, nb,
+                           words, bias);
+        return;
+    }
+    const int big_m = (M + 255) / 256, big_n = (N + 255) / 256;
+    if ((int64_t)big_m * big_n >= 512) {
+        hipLaunchKernelGGL((gemm_fp8_tiles<T, 4, 4>), dim3(big_m * big_n), dim3(256), 0, st, a, b, out, ldo, M, N, nb, words,
+                           bias, big_m, big_n);
+    } else {
+        const int tm = (M + 127) / 128, tn = (N + 127) / 128;
+        hipLaunchKernelGGL((gemm_fp8_tiles<T, 2, 2>), dim3(tm * tn), dim3(256), 0, st, a, b, out, ldo, M, N, nb, words, bias,
+                           tm, tn);
+    }
+}
+}  // namespace
+
+extern "C" int icrl_gemm_fp8(const void* a_pieces, const void* a_scales, const void* b_pieces, const void* b_scales, void* C,
+                             int dtype, int64_t ldc, int M, int N, int K, const float* bias, icrl_stream_t stream) {
+    ICRL_REQUIRE(a_pieces && a_scales && b_pieces && b_scales && C && M > 0 && N > 0 && K > 0, "icrl_gemm_fp8: null operand or empty shape");
+    ICRL_REQUIRE(ldc >= N, "icrl_gemm_fp8: leading dimension ldc < N");
+    ICRL_REQUIRE((reinterpret_cast<uintptr_t>(a_pieces) | reinterpret_cast<uintptr_t>(b_pieces)) % 16 == 0 &&
+                     (reinterpret_cast<uintptr_t>(a_scales) | reinterpret_cast<uintptr_t>(b_scales)) % 4 == 0,
+                 "icrl_gemm_fp8: pieces must be 16-byte aligned, scales 4-byte");
+    ICRL_REQUIRE((int64_t)((M + 127) / 128) * ((N + 127) / 128) <= 0x7FFFFFFF, "icrl_gemm_fp8: output too large");
+    const Operand a{static_cast<const unsigned char*>(a_pieces), static_cast<const unsigned*>(a_scales), (M + 31) / 32};
+    const Operand b{static_cast<const unsigned char*>(b_pieces), static_cast<const unsigned*>(b_scales), (N + 31) / 32};
+    hipStream_t st = icrl::as_stream(stream);
+    switch (dtype) {
+        case ICRL_F32: launch_gemm(a, b, static_cast<float*>(C), ldc, M, N, K, bias, st); break;
+        case ICRL_BF16: launch_gemm(a, b, static_cast<__bf16*>(C), ldc, M, N, K, bias, st); break;
+        case ICRL_F16: launch_gemm(a, b, static_cast<_Float16*>(C), ldc, M, N, K, bias, st); break;
+        default: icrl::set_error("icrl_gemm_fp8: unknown dtype %d", dtype); return ICRL_ERR_ARG;
+    }
+    ICRL_LAUNCH_CHECK();
+    return ICRL_OK;
+}

@@ -1,0 +1,188 @@
+// One row of logits (float32, bf16 or f16, any length) worked on by one workgroup: how the operators that filter,
+// rank and distil a row read it.  Device code for gfx950.
+#pragma once
+#include "icrl_common.h"
+
+namespace icrl {
+
+typedef unsigned long long u64;
+
+template <typename T>
+struct Elem;   // how many fit 16 bytes, and their value in float32 (exact for all three types)
+template <>
+struct Elem<float> {
+    static constexpr int VEC = 4;
+    using Raw = unsigned;
+    static __device__ __forceinline__ float value(Raw r) { return __uint_as_float(r); }
+};
+template <>
+struct Elem<__bf16> {
+    static constexpr int VEC = 8;
+    using Raw = unsigned short;
+    static __device__ __forceinline__ float value(Raw r) { return __uint_as_float((unsigned)r << 16); }
+};
+template <>
+struct Elem<_Float16> {
+    static constexpr int VEC = 8;
+    using Raw = unsigned short;
+    static __device__ __forceinline__ float value(Raw r) { return (float)__builtin_bit_cast(_Float16, r); }
+};
+
+// Where a row's entries are between the passes over it.  PLACE > 0: in registers, at most PLACE vectors of 16 bytes a
+// thread, for operators with a few short passes (every pass is unrolled).  IN_LDS: staged once.  IN_MEMORY: every pass
+// reads the row again, from the caches where it fits them.
+constexpr int IN_MEMORY = 0, IN_LDS = -1;
+
+// A row is cut into one contiguous piece per wave, a multiple of 64 x 16 bytes, and a piece into wave-wide vectors of
+// 16 bytes a lane: reads are 1 KB of consecutive bytes, and (wave, vector, lane, element) is the order of the indices,
+// which the draw and the ranking of ties need.  Rows need no alignment beyond their element's: gfx950 reads 16 bytes
+// from any address.  Places past the row's end hold -inf, or (CANON) a NaN of their own that orders below every entry,
+// the canonical NaN included; CANON also turns every NaN into one and -0 into +0, so that equal entries have equal keys.
+template <typename T, int NT, int PLACE, bool CANON>
+struct Row {
+    static constexpr int VEC = Elem<T>::VEC, NW = NT / 64;
+    using Raw = typename Elem<T>::Raw;
+    static constexpr Raw kNan = sizeof(T) == 4 ? (Raw)0xFFC00000u : (__is_same(T, __bf16) ? (Raw)0xFFC0u : (Raw)0xFE00u);
+    static constexpr Raw kMinusInf = sizeof(T) == 4 ? (Raw)0xFF800000u : (__is_same(T, __bf16) ? (Raw)0xFF80u : (Raw)0xFC00u);
+    static constexpr Raw kMinusZero = (Raw)((Raw)1 << (8 * sizeof(Raw) - 1));
+    static constexpr Raw kFill = CANON ? (Raw)~0u : kMinusInf;
+    struct alignas(16) Pack { Raw e[VEC]; };
+    typedef unsigned Words __attribute__((ext_vector_type(4), aligned(2), may_alias));   // one 16-byte access
+    const T* src;
+    Pack* staged;        // IN_LDS: the workgroup's copy, this thread's first vector
+    int V, vectors;      // vectors: how many per thread
+    int first;           // index of the thread's first entry
+    Pack keep[PLACE > 0 ? PLACE : 1];
+
+    // 16-byte vectors that a workgroup stages for a row of V entries
+    static __host__ __device__ int lds_vectors(int V) { return (V + NT * VEC - 1) / (NT * VEC) * NT; }
+
+    __device__ __forceinline__ Pack read(int i) const {
+        const int at = first + i * 64 * VEC;
+        Pack p;
+        if (at + VEC <= V) {
+            p = __builtin_bit_cast(Pack, *reinterpret_cast<const Words*>(src + at));
+        } else {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                p.e[j] = kFill;
+                if (at + j < V) __builtin_memcpy(&p.e[j], src + at + j, sizeof(Raw));
+            }
+        }
+        return p;
+    }
+    __device__ __forceinline__ Pack canonical(Pack p, int i) const {
+        const int at = first + i * 64 * VEC;
+        if (CANON) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                const float x = Elem<T>::value(p.e[j]);
+                const Raw same = p.e[j] == kMinusZero ? (Raw)0 : p.e[j];
+                p.e[j] = x != x && at + j < V ? kNan : same;
+            }
+        }
+        return p;
+    }
+    __device__ __forceinline__ Pack fetch(int i) const {
+        if constexpr (PLACE == IN_LDS) return staged[i * 64];
+        else return canonical(read(i), i);
+    }
+
+    // lds: lds_vectors(count) vectors if IN_LDS.  No barrier is needed: a thread reads back what it wrote itself.
+    __device__ __forceinline__ void open(const T* row, int count, void* lds) {
+        src = row;
+        V = count;
+        vectors = (count + NT * VEC - 1) / (NT * VEC);
+        const int at = (int)(threadIdx.x >> 6) * vectors * 64 + (int)(threadIdx.x & 63);
+        first = at * VEC;
+        staged = static_cast<Pack*>(lds) + at;
+        if constexpr (PLACE > 0) {
+#pragma unroll
+            for (int i = 0; i < PLACE; ++i)
+                if (i < vectors) keep[i] = canonical(read(i), i);
+        } else if constexpr (PLACE == IN_LDS) {
+            constexpr int AHEAD = 4;   // reads in flight per thread
+            for (int i = 0; i < vectors; i += AHEAD) {
+                Pack p[AHEAD];
+#pragma unroll
+                for (int q = 0; q < AHEAD; ++q)
+                    if (i + q < vectors) p[q] = read(i + q);
+#pragma unroll
+                for (int q = 0; q < AHEAD; ++q)
+                    if (i + q < vectors) staged[(i + q) * 64] = canonical(p[q], i + q);
+            }
+        }
+    }
+
+    // f(vector, index of its first entry) for each of the thread's vectors
+    template <typename F>
+    __device__ __forceinline__ void each_pack(F&& f) const {
+        if constexpr (PLACE > 0) {
+#pragma unroll
+            for (int i = 0; i < PLACE; ++i)
+                if (i < vectors) f(keep[i], first + i * 64 * VEC);
+        } else if constexpr (PLACE == IN_LDS) {
+            for (int i = 0; i < vectors; ++i) f(staged[i * 64], first + i * 64 * VEC);
+        } else {
+            constexpr int AHEAD = 4;
+            for (int i = 0; i < vectors; i += AHEAD) {
+                Pack p[AHEAD];
+#pragma unroll
+                for (int q = 0; q < AHEAD; ++q)
+                    if (i + q < vectors) p[q] = read(i + q);
+#pragma unroll 1
+                for (int q = 0; q < AHEAD; ++q) {
+                    if (i + q < vectors) f(canonical(p[0], i + q), first + (i + q) * 64 * VEC);
+#pragma unroll
+                    for (int s = 0; s + 1 < AHEAD; ++s) p[s] = p[s + 1];   // a queue, not an indexed array: it stays in registers
+                }
+            }
+        }
+    }
+    // f(value, index) for every place of a vector, or of all of them (places past the end included)
+    template <typename F>
+    __device__ __forceinline__ void vector(const Pack& p, int at, F&& f) const {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) f(Elem<T>::value(p.e[j]), at + j);
+    }
+    template <typename F>
+    __device__ __forceinline__ void each(F&& f) const {
+        each_pack([&](const Pack& p, int at) { vector(p, at, f); });
+    }
+};
+
+// Unsigned keys in the order of the values.  -inf: 0x007FFFFF; the canonical NaN below it, places past the end below that.
+constexpr unsigned kKeyNan = 0x003FFFFFu, kKeyMinusInf = 0x007FFFFFu, kKeyFinite = 0x00800000u, kKeyPlusInf = 0xFF800000u;
+__device__ __forceinline__ unsigned order_key(float x) {
+    const int b = __float_as_int(x);
+    return (unsigned)(b ^ ((b >> 31) | (int)0x80000000));
+}
+
+// 2^t for t <= 0 in float64, by the Taylor series of 2^r = e^(r ln 2) on |r| <= 1/2: eleven terms leave
+// 0.3466^12 / 12! = 6e-15.  (The library's exp2 spends several times the instructions on the last two bits.)
+__device__ __forceinline__ double exp2_neg(double t) {
+    const double n = rint(t), r = t - n;
+    constexpr double L = 0.69314718055994530942;
+    double p = 1.0 / 39916800.0;
+    const double y = r * L;
+    p = fma(p, y, 1.0 / 3628800.0);
+    p = fma(p, y, 1.0 / 362880.0);
+    p = fma(p, y, 1.0 / 40320.0);
+    p = fma(p, y, 1.0 / 5040.0);
+    p = fma(p, y, 1.0 / 720.0);
+    p = fma(p, y, 1.0 / 120.0);
+    p = fma(p, y, 1.0 / 24.0);
+    p = fma(p, y, 1.0 / 6.0);
+    p = fma(p, y, 0.5);
+    p = fma(p, y, 1.0);
+    p = fma(p, y, 1.0);
+    return ldexp(p, (int)n);
+}
+
+__device__ __forceinline__ u64 wave_sum_u64(u64 v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    return v;
+}
+
+}  // namespace icrl

@@ -42,6 +42,10 @@ SIGNATURES = {
                                         c_int, c_int, c_int, c_vp]),
     "icrl_absmax_scales": (c_int, [c_vp, c_i64, c_int, c_int, c_vp, c_vp, c_vp, c_vp]),
     "icrl_g0_row_scales": (c_int, [c_vp, c_int, c_vp, c_vp]),
+    "icrl_fp8_piece_bytes": (c_i64, [c_int, c_int]),
+    "icrl_fp8_scale_bytes": (c_i64, [c_int, c_int]),
+    "icrl_cut_fp8": (c_int, [c_vp, c_int, c_i64, c_int, c_int, c_vp, c_vp, c_vp]),
+    "icrl_gemm_fp8": (c_int, [c_vp] * 5 + [c_int, c_i64, c_int, c_int, c_int, c_vp, c_vp]),
     "icrl_sum_slabs": (c_int, [c_vp, c_i64, c_int, c_i64, c_vp, c_int, c_vp]),
     "icrl_chain_seg_workspace_floats": (c_i64, [c_int]),
     "icrl_lstm_chain_fwd_seg": (c_int, [c_vp, c_vp] + [c_int] * 6 + [c_vp] * 6),
@@ -92,6 +96,12 @@ SIGNATURES = {
     "icrl_sample_tokens_lstm_cell": (c_int, [c_vp, c_i64, c_int, c_int, c_int, c_vp, c_vp, c_i64, c_vp, c_i64, c_vp, c_vp,
                                              c_vp, c_i64, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp]),
     "icrl_policy_rollout_rounds": (c_int, [c_vp] * 6 + [c_i64] + [c_int] * 5 + [c_vp] * 10),
+    "icrl_sample_tokens_filtered": (c_int, [c_vp, c_int, c_i64, c_int, c_int, c_vp, c_vp, c_f64, c_vp, c_int, c_vp, c_f64,
+                                            c_vp, c_f64, c_vp, c_i64, c_vp, c_i64, c_vp]),
+    "icrl_topk_lse_rows": (c_int, [c_vp, c_int, c_i64, c_int, c_int, c_int, c_f64, c_vp, c_vp, c_vp, c_vp]),
+    "icrl_distill_loss": (c_int, [c_vp, c_int, c_i64, c_int, c_int, c_vp, c_vp, c_int, c_vp, c_f64, c_vp, c_vp, c_vp, c_vp,
+                                  c_i64, c_vp]),
+    "icrl_distill_grad": (c_int, [c_vp, c_int, c_i64, c_int, c_int, c_vp, c_vp, c_int, c_f64, c_vp, c_vp, c_vp, c_i64, c_vp]),
     "icrl_policy_dlogits": (c_int, [c_vp, c_vp, c_int, c_int, c_vp, c_i64, c_vp, c_vp]),
     "icrl_chain_sync_bytes": (c_i64, []),
     "icrl_lstm_chain_fwd": (c_int, [c_vp, c_vp, c_int, c_int, c_int, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp]),
@@ -108,8 +118,9 @@ SIGNATURES = {
 }
 
 SAMPLE, GREEDY, FORCED = 0, 1, 2
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}   # ICRL_F32 / ICRL_BF16 / ICRL_F16
 EMIT_DLOGITS = 16   # or-ed into SAMPLE / FORCED: the probs output receives onehot(token) - softmax
-ABI_VERSION = 4
+ABI_VERSION = 5
 
 _lib = None
 
@@ -238,6 +249,40 @@ def _chain_shapes(who, n, p0, n_calls, gates, xproj=None, h_emit=None, saved=Non
         need(work, chain_seg_workspace_floats(segments), "work")
 
 
+def _dtype_code(t):
+    assert t.dtype in DTYPES, "float32, bfloat16 or float16 expected, got %s" % t.dtype
+    return DTYPES[t.dtype]
+
+
+def _row_stride(t):
+    """Row stride of a 2-D tensor whose rows are contiguous (of a single row, or a single column: any that is valid)."""
+    assert t.dim() == 2 and (t.stride(1) == 1 or t.shape[1] == 1), "rows must be contiguous"
+    return t.stride(0) if t.shape[0] > 1 and t.stride(0) >= t.shape[1] else _no_overlap(t)
+
+
+def _no_overlap(t):
+    assert t.shape[0] <= 1, "rows must not overlap"
+    return t.shape[1]
+
+
+def _on_current_device(*tensors):
+    """Launches go to the current device's stream: every operand must live there."""
+    current = None
+    for t in tensors:
+        if isinstance(t, torch.Tensor):
+            assert t.is_cuda, "the HIP kernels take device tensors"
+            if current is None:
+                current = torch.cuda.current_device() if _raw_device is None else _raw_device()
+            assert t.get_device() == current, "operand on cuda:%d, the current device is cuda:%d" % (t.get_device(), current)
+
+
+def _vector(t, n, dtype, name):
+    """An optional contiguous vector of n entries."""
+    assert t is None or (t.dtype == dtype and t.is_contiguous() and t.numel() == n), \
+        "%s must be %d contiguous %s" % (name, n, dtype)
+    return _ptr(t)
+
+
 def _f32c(t):
     assert t.dtype == torch.float32 and t.is_contiguous(), (t.dtype, t.is_contiguous())
     return t
@@ -326,6 +371,43 @@ def gemm_f16x2(a_pieces, a_descale, b_pieces, b_descale, out, k, bias=None):
         rc = load().icrl_gemm_f16x2(_ptr(a_pieces), _ptr(a_descale), _ptr(b_pieces), _ptr(b_descale), _ptr(out),
                                     out.stride(0), m, n, k, _ptr(bias), _stream())
     _check(rc, "icrl_gemm_f16x2")
+    return out
+
+
+def fp8_pieces(rows, k, device):
+    """Buffers (pieces, scales) for a [rows, k] operand of gemm_fp8; cut_fp8 writes them whole."""
+    assert rows > 0 and k > 0, "an 8-bit operand needs rows and columns"
+    return (torch.empty(load().icrl_fp8_piece_bytes(rows, k), dtype=torch.uint8, device=device),
+            torch.empty(load().icrl_fp8_scale_bytes(rows, k), dtype=torch.uint8, device=device))
+
+
+def _fp8_operand(pieces, scales, rows, k):
+    assert pieces.dtype == scales.dtype == torch.uint8 and pieces.is_contiguous() and scales.is_contiguous()
+    assert pieces.numel() >= load().icrl_fp8_piece_bytes(rows, k) > 0 and scales.numel() >= load().icrl_fp8_scale_bytes(rows, k), \
+        "8-bit buffers too small for [%d, %d]" % (rows, k)
+
+
+def cut_fp8(x, pieces, scales):
+    """Cuts x [rows, k] (float32, bfloat16 or float16, rows contiguous) into e4m3 codes with one power-of-two scale per
+    row and block of 128 along k, in the matrix instruction's fragment order (buffers from fp8_pieces)."""
+    rows, k = x.shape
+    _on_current_device(x, pieces, scales)
+    _fp8_operand(pieces, scales, rows, k)
+    _check(load().icrl_cut_fp8(_ptr(x), _dtype_code(x), _row_stride(x), rows, k, _ptr(pieces), _ptr(scales), _stream()),
+           "icrl_cut_fp8")
+
+
+def gemm_fp8(a_pieces, a_scales, b_pieces, b_scales, out, k, bias=None):
+    """out[M, N] = A . B^T (+ bias) from operands cut by cut_fp8 as [M, k] and [N, k]; out float32, bfloat16 or float16,
+    float32 sums, one rounding at the end."""
+    m, n = out.shape
+    _on_current_device(a_pieces, a_scales, b_pieces, b_scales, out, bias)
+    _fp8_operand(a_pieces, a_scales, m, k)
+    _fp8_operand(b_pieces, b_scales, n, k)
+    with _Timed("gemm_fp8", 2.0 * m * n * k, m * k + k * n + float(out.element_size()) * m * n):
+        rc = load().icrl_gemm_fp8(_ptr(a_pieces), _ptr(a_scales), _ptr(b_pieces), _ptr(b_scales), _ptr(out), _dtype_code(out),
+                                  _row_stride(out), m, n, k, _vector(bias, n, torch.float32, "bias"), _stream())
+    _check(rc, "icrl_gemm_fp8")
     return out
 
 
@@ -483,6 +565,96 @@ def topk_rows(logits, k):
     _check(load().icrl_topk_rows(_ptr(logits), logits.stride(0), n, v, k, _ptr(values), _ptr(indices), _stream()),
            "icrl_topk_rows")
     return values, indices
+
+
+def sample_tokens_filtered(logits, tokens_out, token_stride, uniforms, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
+                           log_prob=None, log_prob_stride=1):
+    """One token per row of logits [N, V] (float32, bfloat16 or float16, rows contiguous) from the softmax at
+    `temperature` restricted to the top_k largest entries (0: all), of those the shortest prefix that holds top_p of the
+    mass, of those the entries with at least min_p of the largest one's probability; uniforms [N] float64 decide.  Each
+    setting is a number or an [N] tensor (float32; top_k int32).  Temperature 0: the first largest entry.  token -1 and
+    log_prob NaN: the row holds a NaN or nothing above -inf, or its settings are out of range."""
+    n, v = logits.shape
+    _on_current_device(logits, tokens_out, uniforms, temperature, top_k, top_p, min_p, log_prob)
+    assert tokens_out.dtype == torch.int64 and _holds(tokens_out, n, token_stride), "tokens_out: int64, one place per row"
+    assert log_prob is None or (log_prob.dtype == torch.float32 and _holds(log_prob, n, log_prob_stride)), \
+        "log_prob: float32, one place per row"
+    assert uniforms is not None
+
+    def setting(value, dtype, name):
+        if torch.is_tensor(value):
+            return _vector(value, n, dtype, name), 0
+        return None, value
+
+    t_rows, t = setting(temperature, torch.float32, "temperature")
+    k_rows, k = setting(top_k, torch.int32, "top_k")
+    p_rows, p = setting(top_p, torch.float32, "top_p")
+    m_rows, m = setting(min_p, torch.float32, "min_p")
+    _check(load().icrl_sample_tokens_filtered(_ptr(logits), _dtype_code(logits), _row_stride(logits), n, v,
+                                              _vector(uniforms, n, torch.float64, "uniforms"), t_rows, float(t), k_rows,
+                                              min(int(k), v), p_rows, float(p), m_rows, float(m), _ptr(tokens_out),
+                                              token_stride, _ptr(log_prob), log_prob_stride, _stream()),
+           "icrl_sample_tokens_filtered")
+
+
+def _holds(t, n, stride):
+    """Whether a buffer that starts at t's first element has n places `stride` elements apart."""
+    return stride >= 1 and t.untyped_storage().nbytes() // t.element_size() - t.storage_offset() >= (n - 1) * stride + 1
+
+
+def topk_lse_rows(logits, values, indices, lse=None, *, temperature=1.0):
+    """values / indices [N, k] = the k <= 1024 largest entries of each row of logits [N, V] (float32, bfloat16 or
+    float16), descending, ties by lowest index; lse [N] (optional) = log sum e^(x / temperature) over the row."""
+    n, v = logits.shape
+    k = values.shape[1]
+    _on_current_device(logits, values, indices, lse)
+    assert values.shape == indices.shape == (n, k) and indices.dtype == torch.int64 and indices.is_contiguous()
+    _check(load().icrl_topk_lse_rows(_ptr(logits), _dtype_code(logits), _row_stride(logits), n, v, k, float(temperature),
+                                     _ptr(_f32c(values)), _ptr(indices), _vector(lse, n, torch.float32, "lse"), _stream()),
+           "icrl_topk_lse_rows")
+
+
+def _distill_operands(logits, teacher_values, teacher_indices, dlogits, stats):
+    n = logits.shape[0]
+    k = teacher_values.shape[1]
+    assert teacher_values.shape == teacher_indices.shape == (n, k) and teacher_indices.dtype == torch.int64
+    assert teacher_indices.is_contiguous()
+    if dlogits is not None:
+        assert dlogits.shape == logits.shape and dlogits.dtype == logits.dtype, "dlogits must be shaped and typed like the logits"
+        assert dlogits.data_ptr() != logits.data_ptr() or _row_stride(dlogits) == _row_stride(logits)
+    assert stats is None or (stats.dtype == torch.float64 and stats.is_contiguous() and stats.numel() == 4 * n), \
+        "stats must be %d contiguous float64" % (4 * n)
+    return n, k
+
+
+def distill_loss(logits, teacher_values, teacher_indices, row_loss, *, teacher_lse=None, temperature=1.0, row_weight=None,
+                 stats=None, dlogits=None):
+    """row_loss [N] = row_weight * the divergence of softmax(logits / temperature) from a teacher known by its k largest
+    logits (teacher_values float32, teacher_indices int64, [N, k], as topk_lse_rows leaves them; a negative index is an
+    absent entry).  With teacher_lse [N] (the teacher's log-normaliser at this temperature) the words outside the list
+    are one more word; without it the teacher is renormalised over the list.  dlogits (optional, may be logits itself):
+    the gradient, written by the same pass; stats (optional, [N, 4] float64): what distill_grad needs instead."""
+    n, k = _distill_operands(logits, teacher_values, teacher_indices, dlogits, stats)
+    _on_current_device(logits, teacher_values, teacher_indices, row_loss, teacher_lse, row_weight, stats, dlogits)
+    assert row_loss is not None
+    _check(load().icrl_distill_loss(_ptr(logits), _dtype_code(logits), _row_stride(logits), n, logits.shape[1],
+                                    _ptr(_f32c(teacher_values)), _ptr(teacher_indices), k,
+                                    _vector(teacher_lse, n, torch.float32, "teacher_lse"), float(temperature),
+                                    _vector(row_weight, n, torch.float32, "row_weight"),
+                                    _vector(row_loss, n, torch.float32, "row_loss"), _ptr(stats), _ptr(dlogits),
+                                    0 if dlogits is None else _row_stride(dlogits), _stream()), "icrl_distill_loss")
+
+
+def distill_grad(logits, teacher_values, teacher_indices, stats, dlogits, *, temperature=1.0, row_weight=None):
+    """The gradient of distill_loss from the stats it left; row_weight may be another (rows that had weight 0 keep
+    gradient 0).  dlogits may be logits itself."""
+    assert stats is not None and dlogits is not None
+    n, k = _distill_operands(logits, teacher_values, teacher_indices, dlogits, stats)
+    _on_current_device(logits, teacher_values, teacher_indices, row_weight, stats, dlogits)
+    _check(load().icrl_distill_grad(_ptr(logits), _dtype_code(logits), _row_stride(logits), n, logits.shape[1],
+                                    _ptr(_f32c(teacher_values)), _ptr(teacher_indices), k, float(temperature), _ptr(stats),
+                                    _vector(row_weight, n, torch.float32, "row_weight"), _ptr(dlogits),
+                                    _row_stride(dlogits), _stream()), "icrl_distill_grad")
 
 
 def policy_dlogits(probs, dlogits, tokens, token_stride, coef):

@@ -31,7 +31,7 @@ typedef void* icrl_stream_t;
 #define ICRL_ERR_HIP (-2)     /* a HIP runtime call failed */
 #define ICRL_ERR_TIMEOUT (-3) /* a chain kernel gave up waiting for a peer workgroup */
 
-#define ICRL_ABI_VERSION 4
+#define ICRL_ABI_VERSION 5
 
 int icrl_abi_version(void);
 const char* icrl_last_error(void);
@@ -138,6 +138,28 @@ int icrl_gemm_f16x2s_splitk_tile(const float* A, int64_t lda, int a_kmajor, cons
 int icrl_absmax_scales(const float* x, int64_t ld, int rows, int cols, float* row_scale, float* col_scale,
                        unsigned* work, icrl_stream_t stream);
 int icrl_g0_row_scales(const float* log_prob, int count, float* scale, icrl_stream_t stream);
+
+/* Element types of the entry points that take more than float32 (`dtype`). */
+#define ICRL_F32 0
+#define ICRL_BF16 1
+#define ICRL_F16 2
+
+/* C = A . B^T (+ bias) on 8-bit operands (e4m3) with one power-of-two scale for each row and block of 128 along k, on
+ * v_mfma_scale_f32_32x32x64_f8f6f4 with float32 sums: for a network that is served, whose vocabulary weight
+ * (models.py:82) is then a quarter of its float32 size.  icrl_cut_fp8 cuts x [rows, K] (row stride ld entries, dtype
+ * ICRL_F32 / BF16 / F16, any alignment): scale = the smallest power of two that keeps the block's largest magnitude
+ * within 448, codes = the scaled values (exact) rounded to nearest even, so an entry is off by at most 2^-4 of itself, or
+ * by 2^-10 of the scale where it is below 2^-6 of it.  Scales below 2^-127 are 2^-127; a block with a NaN or an infinity
+ * has scale NaN, and its row's results are NaN.  pieces / scales: icrl_fp8_piece_bytes / icrl_fp8_scale_bytes(rows, K)
+ * bytes (16- / 4-byte aligned), written whole, the padding to 32 rows and 128 k with zeros.
+ * icrl_gemm_fp8: C [M, N] (row stride ldc, dtype any of the three) from A cut as (M, K) and B as (N, K), plus
+ * bias[n] (optional, float32). */
+int64_t icrl_fp8_piece_bytes(int rows, int K);
+int64_t icrl_fp8_scale_bytes(int rows, int K);
+int icrl_cut_fp8(const void* x, int dtype, int64_t ld, int rows, int K, void* pieces, void* scales,
+                 icrl_stream_t stream);
+int icrl_gemm_fp8(const void* a_pieces, const void* a_scales, const void* b_pieces, const void* b_scales, void* C,
+                  int dtype, int64_t ldc, int M, int N, int K, const float* bias, icrl_stream_t stream);
 
 /* out[i] = (accumulate ? out[i] : 0) + sum_z slabs[z*slab_stride + i], i < count (count % 4 == 0) */
 int icrl_sum_slabs(const float* slabs, int64_t slab_stride, int splits, int64_t count, float* out,
@@ -303,6 +325,55 @@ int icrl_policy_rollout_rounds(const void* w_pieces, const float* w_descale, con
  * trainers.py:96.  k <= 64, V <= 16384. */
 int icrl_topk_rows(const float* logits, int64_t ld_logits, int N, int V, int k, float* values,
                    int64_t* indices, icrl_stream_t stream);
+
+/* icrl_sample_tokens' draw from a filtered and tempered distribution; no counterpart in the reference, whose rollout
+ * samples the plain softmax (trainers.py:444-458).  One row of logits[N, V] (any of the three dtypes, row stride
+ * ld_logits, any alignment, V <= 4194304) and one uniform double per row:
+ *   order: larger logit first, equal ones by lowest index; weight w = e^((x - max) / temperature);
+ *   top_k: the first top_k entries (0 = all);  top_p: of those, the shortest prefix that holds at least top_p of their
+ *   weight, and never fewer than one;  min_p: of those, the entries with w >= min_p (the largest has w = 1).
+ *   token = the first entry in vocabulary order at which the running sum of the remaining weights exceeds u times
+ *   their sum (u below 0 or from 1 on: the first or last one with weight);  log_prob = log(w / that sum).
+ * temperature 0: the first largest entry, log_prob 0.  Each setting is one value for all rows, or (pointer not null) an
+ * array of N, which then counts.  Entries of -inf are never drawn; if there are entries of +inf only they are.  A row
+ * that holds a NaN or no entry above -inf, or whose settings are out of range (temperature negative or not finite,
+ * top_k negative, top_p or min_p outside [0, 1], u NaN), draws nothing: token -1, log_prob NaN.
+ * Weights are whole multiples of 2^-S of the largest (S = 62 - ceil(log2 V), at most 51), so sums are exact and the
+ * result does not depend on how a row is split. */
+int icrl_sample_tokens_filtered(const void* logits, int dtype, int64_t ld_logits, int N, int V,
+                                const double* uniforms, const float* temperature_rows, double temperature,
+                                const int32_t* top_k_rows, int top_k, const float* top_p_rows, double top_p,
+                                const float* min_p_rows, double min_p, int64_t* tokens_out,
+                                int64_t token_stride, float* log_prob, int64_t log_prob_stride,
+                                icrl_stream_t stream);
+
+/* icrl_topk_rows for any of the three dtypes, V <= 4194304 and k <= 1024, with the row's log-normaliser: values
+ * [N, k] and indices [N, k] of the k largest entries in descending order, ties by lowest index (NaN after -inf);
+ * lse (optional) [N] = log sum e^(x / temperature) over the whole row (NaN if the row holds one).  What a teacher
+ * leaves for icrl_distill_loss. */
+int icrl_topk_lse_rows(const void* logits, int dtype, int64_t ld_logits, int N, int V, int k, double temperature,
+                       float* values, int64_t* indices, float* lse, icrl_stream_t stream);
+
+/* Distillation from a teacher's top logits (icrl_topk_lse_rows); no counterpart in the reference, whose policy
+ * pre-training has captions only (trainers.py:202-257).  Per row, with p = softmax(logits / temperature) and the
+ * listed words' teacher probabilities q_j:
+ *   teacher_lse given: q_j = e^(value_j / temperature - teacher_lse), and the words outside the list count as one more
+ *     word with q_r = max(0, 1 - sum q_j) and p_r = their p together (left out where the policy has no mass there);
+ *   teacher_lse null: q = softmax(value / temperature) over the list.
+ *   row_loss = row_weight * (sum_j q_j log(q_j / p_j) + q_r log(q_r / p_r));
+ *   dlogits (optional; same dtype as logits, which it may be itself) = its gradient.
+ * teacher_values / teacher_indices: [N, k], k <= 1024, V <= 262144; a negative index is an absent entry (its value is
+ * not read), an index >= V or one that occurs twice in a row makes that row's results NaN; a row without entries has
+ * loss and gradient 0.  row_weight (optional) [N]; rows of weight 0 are not read, their results are zeros.  stats
+ * (optional): 4 N doubles for icrl_distill_grad, which writes the gradient later, when the rows' weights may be others
+ * (rows of weight 0 in the forward call keep gradient zero). */
+int icrl_distill_loss(const void* logits, int dtype, int64_t ld_logits, int N, int V, const float* teacher_values,
+                      const int64_t* teacher_indices, int k, const float* teacher_lse, double temperature,
+                      const float* row_weight, float* row_loss, double* stats, void* dlogits, int64_t ld_dlogits,
+                      icrl_stream_t stream);
+int icrl_distill_grad(const void* logits, int dtype, int64_t ld_logits, int N, int V, const float* teacher_values,
+                      const int64_t* teacher_indices, int k, double temperature, const double* stats,
+                      const float* row_weight, void* dlogits, int64_t ld_dlogits, icrl_stream_t stream);
 
 /* d logits for the policy-gradient term from the saved softmax (dlogits may alias probs):
  * g[r, k] = coef[r] * ((k == token[r]) - p[r, k]),  coef = dLoss/dlog_prob; coef NULL = ones (the
