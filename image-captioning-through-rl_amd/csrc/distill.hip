@@ -108,7 +108,7 @@ __global__ __launch_bounds__(NT) void distill_kernel(const T* logits, int64_t ld
         return;
     }
     Row<T, NT, NV, false> row;
-    row.open(src, V, nullptr);
+    row.open(src, V);
     const int words = (V + 31) / 32;
     float* at_listed = reinterpret_cast<float*>(bits + words);
     for (int w = tid; w < words; w += NT) bits[w] = 0;
@@ -230,7 +230,7 @@ __global__ __launch_bounds__(NT) void distill_grad_kernel(const T* logits, int64
     const double log_z = stats[4 * (int64_t)r], teacher = stats[4 * (int64_t)r + 1], W = stats[4 * (int64_t)r + 2],
                  W_out = stats[4 * (int64_t)r + 3];
     Row<T, NT, NV, false> row;
-    row.open(src, V, nullptr);
+    row.open(src, V);
     const double g = (double)weight * per_t;
     for (int j = tid; j < k; j += NT) {
         const int64_t i = ti[j];

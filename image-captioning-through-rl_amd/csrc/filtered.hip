@@ -1,13 +1,18 @@
 // Rows of logits ranked and filtered: token sampling with temperature, top-k, top-p and min-p, and the k largest
 // entries of a row with its log-normaliser.  One workgroup per row.
 //
-// Both need the same thing, a CUT of the row's order (larger value first, ties by lowest index): the entries that come
-// no later than a certain one.  An entry's place in that order is its composite, (order key of the value) << 32 | ~index,
-// so a cut is one 64-bit number and "kept" is composite >= cut; top-k is the cut after k entries and top-p the cut after
-// the shortest prefix with the wanted mass.  A cut is found from a histogram of the row over 2048 equal value ranges
-// (counts for top-k, masses for top-p), which names the range the cut falls into; the few entries of that range are
-// sorted exactly.  Ranges with more entries than threads (many equal values) are refined by three radix passes over
-// the keys instead.
+// A row's order is: larger value first, ties by lowest index.  An entry's place in it is its composite, (order key of the
+// value) << 32 | ~index, and what a filter keeps is always a beginning of the order, composite >= cut.
+//
+// What bounds these operators is not memory but how often a row's entries pass through the one CU that works on it (a
+// row of 10 000 costs 0.07 us for every instruction per entry), so passes are few and short, and everything else is done
+// on lists of at most a thread per entry:
+//   - The k-th largest of the threads' own maxima is a lower bound of the k-th largest entry, and hardly more than k
+//     entries reach it.  They are collected and ranked; filters that start from a top-k never look at the row again.
+//   - min-p alone is a bound itself.  top-p alone needs the whole row's mass, then tries the same short list.
+//   - Where the list does not reach (a flat distribution's nucleus, or more ties than threads), a histogram over 2048
+//     value ranges names the range that the cut falls into, and only that range is ranked, or refined by radix passes
+//     over its keys when even it is too long.
 //
 // Masses are 64-bit integers, multiples of 2^-S of the row's largest weight with S = 62 - ceil(log2 V) (at most 51):
 // integer sums have no order, so atomics and any split of the row give the same bits, and 2^-45 of the largest weight
@@ -25,16 +30,22 @@ constexpr int BINS = 2048;
 
 template <int NT>
 struct Shared {
-    u64 hist[BINS];           // histogram; afterwards the list of entries that is sorted
+    u64 hist[BINS];           // histogram; afterwards, or instead, the list of entries that is ranked
     u64 part[NT / 64 + 1];    // per-wave sums
     unsigned key_lo, key_hi;
     int count, bin, index;
     u64 above, cut, total;
     float red[NT / 64];
     int flag;
+    float bound;
 };
 
 __device__ __forceinline__ u64 composite(unsigned key, int index) { return (u64)key << 32 | (unsigned)~index; }
+__device__ __forceinline__ float value_of(u64 c) {
+    const unsigned key = (unsigned)(c >> 32);
+    return __uint_as_float(key ^ ((key >> 31) ? 0x80000000u : 0xFFFFFFFFu));
+}
+__device__ __forceinline__ int index_of(u64 c) { return (int)~(unsigned)c; }
 
 // Weights of one row: e^((x - top) / T) as multiples of 2^-S.
 struct Weights {
@@ -245,9 +256,7 @@ __device__ __forceinline__ u64 find_cut(const R& row, Shared<NT>& sm, u64 from, 
         c = block_sort<NT>(c, sm.hist);
         u64 a = 0;
         if (c != 0) {
-            const unsigned key = (unsigned)(c >> 32);
-            const float x = __uint_as_float(key ^ ((key >> 31) ? 0x80000000u : 0xFFFFFFFFu));
-            a = amount(x);
+            a = amount(value_of(c));
         }
         const u64 before = block_prefix<NT>(a, sm);
         if (before < need && before + a >= need) sm.cut = c;
@@ -286,13 +295,88 @@ __device__ __forceinline__ u64 find_cut(const R& row, Shared<NT>& sm, u64 from, 
         __syncthreads();
     }
     // the entries with this key, in index order, until they reach what is left
-    const float x = __uint_as_float(lo ^ ((lo >> 31) ? 0x80000000u : 0xFFFFFFFFu));
-    const u64 each = amount(x);
+    const u64 each = amount(value_of((u64)lo << 32));
     auto tie = [&](float y, int i) { const unsigned key = order_key(y); return (u64)(key == lo && kept(key, i)); };
     wave_totals<NT>(row, sm, tie);
     const int last = locate<NT>(row, sm, (need + each - 1) / each - 1, tie);
     __syncthreads();
     return composite(lo, last);
+}
+
+// A value that at least k entries of the row reach (k <= NT), not far below the k-th largest: the k-th largest of the
+// threads' own maxima, cut to its key's upper 16 bits.  One wave finds it, a bit at a time.  -inf: fewer than k threads
+// hold an entry above it.
+template <int NT>
+__device__ __forceinline__ float bound_of(float own_max, int k, Shared<NT>& sm) {
+    unsigned* keys = reinterpret_cast<unsigned*>(sm.hist);
+    __syncthreads();
+    keys[threadIdx.x] = order_key(own_max + 0.f);
+    __syncthreads();
+    if (threadIdx.x < 64) {
+        unsigned key[NT / 64], t = 0;
+#pragma unroll
+        for (int i = 0; i < NT / 64; ++i) key[i] = keys[threadIdx.x + 64 * i] >> 16;
+        for (unsigned bit = 0x8000u; bit; bit >>= 1) {
+            int reached = 0;
+#pragma unroll
+            for (int i = 0; i < NT / 64; ++i) reached += __popcll(__ballot(key[i] >= (t | bit)));
+            if (reached >= k) t |= bit;
+        }
+        if (threadIdx.x == 0) {
+            t <<= 16;
+            // between two upper halves lies -inf's: what rounds down to it or below says nothing
+            sm.bound = t <= kKeyMinusInf ? -INFINITY : value_of((u64)t << 32);
+        }
+    }
+    __syncthreads();
+    return sm.bound;
+}
+
+// Composites of the entries >= bound (> -inf) into sm.hist, at most `room` of them; returns how many there are.
+template <int NT, typename R>
+__device__ __forceinline__ int collect(const R& row, Shared<NT>& sm, float bound, int room) {
+    __syncthreads();
+    if (threadIdx.x == 0) sm.count = 0;
+    __syncthreads();
+    row.each_pack([&](const typename R::Pack& p, int at) {
+        float most = -INFINITY;
+        row.vector(p, at, [&](float x, int) { most = fmaxf(most, x); });
+        if (most >= bound)
+            row.vector(p, at, [&](float x, int i) {
+                if (x >= bound) {
+                    const int to = atomicAdd(&sm.count, 1);
+                    if (to < room) sm.hist[to] = composite(order_key(x + 0.f), i);
+                }
+            });
+    });
+    __syncthreads();
+    return sm.count;
+}
+
+// Sorts the n <= NT composites in sm.hist: thread i gets the i-th of the order (0 past the end).  Short lists are ranked
+// by comparing all with all (n / 2 reads of two entries each, 0.5 us at n = 100 against 2.8 us for the sort).
+template <int NT>
+__device__ __forceinline__ u64 ranked(int n, Shared<NT>& sm) {
+    const int tid = threadIdx.x;
+    if (n <= 256 && n < BINS / 2) {
+        u64* out = sm.hist + BINS / 2;
+        if (tid == 0) sm.hist[n] = 0;   // an even number of entries to read
+        __syncthreads();
+        if (tid < n) {
+            const u64 mine = sm.hist[tid];
+            const ulonglong2* two = reinterpret_cast<const ulonglong2*>(sm.hist);
+            int rank = 0;
+            for (int j = 0; j < (n + 1) / 2; ++j) {
+                const ulonglong2 o = two[j];
+                rank += (o.x > mine) + (o.y > mine);
+            }
+            out[rank] = mine;
+        }
+        __syncthreads();
+        return tid < n ? out[tid] : 0;
+    }
+    const u64 c = tid < n ? sm.hist[tid] : 0;
+    return block_sort<NT>(c, sm.hist);
 }
 
 // ---------------------------------------------------------------------------------------------- sampling
@@ -301,6 +385,10 @@ struct Setting {   // one filter setting: a value for each row, or one for all o
     double all;
     __device__ __forceinline__ double at(int r) const { return rows ? (double)rows[r] : all; }
 };
+
+// The draw from a list: thread i holds kept entry i's index and weight (0: none).  Every kept entry adds up the weights of
+// those that come no later in the vocabulary; the one whose sum first exceeds the target is drawn.
+struct Kept { u64 w; unsigned index, pad; };
 
 template <typename T, int NT, int PLACE>
 __global__ __launch_bounds__(NT) void sample_filtered_kernel(const T* __restrict__ logits, int64_t ld, int V, int S,
@@ -311,18 +399,18 @@ __global__ __launch_bounds__(NT) void sample_filtered_kernel(const T* __restrict
                                                              float* __restrict__ log_prob, int64_t lp_stride) {
     __shared__ Shared<NT> sm;
     const int r = blockIdx.x, tid = threadIdx.x;
-    Row<T, NT, PLACE, true> row;
-    extern __shared__ __attribute__((aligned(16))) unsigned char staged[];
-    row.open(logits + (int64_t)r * ld, V, staged);
+    Row<T, NT, PLACE, false> row;
+    row.open(logits + (int64_t)r * ld, V);
     const double temp = temperature.at(r), top_p = top_p_in.at(r), min_p = min_p_in.at(r), u = uniforms[r];
     const int top_k = top_k_rows ? top_k_rows[r] : top_k_all;
     if (tid == 0) sm.flag = 0;
     float best = -INFINITY;
     bool nan = false;
-    row.each([&](float x, int i) {
+    row.each([&](float x, int) {
         best = fmaxf(best, x);                       // fmaxf passes over NaN
-        nan |= x != x && i < V;
+        nan |= x != x;
     });
+    const float own = best;
     best = block_max<NT>(best, sm.red);
     if (nan) sm.flag = 1;
     __syncthreads();
@@ -335,54 +423,127 @@ __global__ __launch_bounds__(NT) void sample_filtered_kernel(const T* __restrict
         }
         return;
     }
-    // with an entry of +inf only the entries of +inf have weight (all the same)
-    const unsigned least = best == INFINITY ? kKeyPlusInf : kKeyFinite;
-    u64 cut = (u64)least << 32;
     if (temp == 0.0 || top_k == 1 || top_p == 0.0) {   // the first largest entry
-        wave_totals<NT>(row, sm, [&](float x, int) { return (u64)(x == best); });
-        const int at = locate<NT>(row, sm, 0, [&](float x, int) { return (u64)(x == best); });
+        if (tid == 0) sm.index = V;
+        __syncthreads();
+        if (own == best) {
+            int first = V;
+            row.each([&](float x, int i) { first = x == best ? min(first, i) : first; });
+            atomicMin(&sm.index, first);
+        }
+        __syncthreads();
         if (tid == 0) {
-            tokens[r * token_stride] = at;
+            tokens[r * token_stride] = sm.index;
             if (log_prob) log_prob[r * lp_stride] = 0.f;
         }
         return;
     }
     const Weights weight{best, 1.4426950408889634074 / temp, S};
-    const float reach = (float)(S * 0.6931471805599453 * temp);   // entries further below the top weigh nothing
-    if (top_k > 0 && top_k < V) {
+    const double floor_z = min_p > 0.0 ? log(min_p) * temp : -INFINITY;   // w >= min_p as x - best >= T log(min_p)
+    auto write = [&](int token, float x, u64 total) {
+        tokens[r * token_stride] = token;
+        if (log_prob) {
+            const double z = x == best ? 0.0 : ((double)x - (double)best) / temp;
+            log_prob[r * lp_stride] = (float)(z - log(ldexp((double)total, -S)));
+        }
+    };
+    auto target_of = [&](u64 total) {
+        const double want = u * (double)total;
+        const u64 target = want > 0.0 ? (u64)fmin(want, 0x1p63) : 0;
+        return target < total ? target : total - 1;
+    };
+    auto prefix_mass = [&](u64 total) {   // what top_p asks for
+        const double w = ceil(top_p * (double)total);
+        const u64 want = w < 1.0 ? 1 : (u64)w;
+        return want < total ? want : total;
+    };
+    const bool by_k = top_k > 0 && top_k < V, by_p = top_p < 1.0;
+
+    // ---- the short list: entries no smaller than a bound that everything kept reaches
+    constexpr int LIST = NT / 2;   // longest list drawn from
+    float bound = -INFINITY;
+    bool guess = false;            // whether the bound is only likely to reach far enough
+    if (by_k) {
+        if (top_k <= NT / 4) bound = bound_of<NT>(own, top_k, sm);
+    } else if (min_p > 0.0) {
+        const double z = (double)best + floor_z;
+        bound = (float)z;
+        if ((double)bound > z) bound = nextafterf(bound, -INFINITY);
+        if (best == INFINITY) bound = INFINITY;
+    } else if (by_p) {
+        bound = bound_of<NT>(own, NT / 8, sm);
+        guess = true;
+    }
+    u64 row_mass = 0;   // of the whole row, where top_p counts from it
+    if (bound > -INFINITY) {
+        const int n = collect<NT>(row, sm, bound, LIST);
+        if (n <= LIST) {
+            bool whole = true;
+            u64 c = 0;
+            if (by_k || by_p) c = ranked<NT>(n, sm);
+            else if (tid < n) c = sm.hist[tid];
+            if (by_k && tid >= top_k) c = 0;
+            const float x = c ? value_of(c) : 0.f;
+            u64 w = c ? weight(x) : 0;
+            if (by_p) {
+                const u64 before = block_prefix<NT>(w, sm);
+                const u64 listed = sm.total;
+                if (!by_k) row_mass = wave_totals<NT>(row, sm, [&](float y, int) { return weight(y); });
+                const u64 want = prefix_mass(by_k ? listed : row_mass);
+                whole = listed >= want || !guess;
+                if (before >= want) w = 0;
+            }
+            if (whole) {
+                if (c && x != best && (double)x - (double)best < floor_z) w = 0;
+                // kept entries side by side, then everyone against everyone
+                Kept* kept = reinterpret_cast<Kept*>(sm.hist);
+                static_assert(sizeof(Kept) * LIST <= sizeof(sm.hist), "the kept list fits the histogram's place");
+                __syncthreads();
+                if (tid == 0) { sm.count = 0; sm.cut = 0; }
+                __syncthreads();
+                if (w) {
+                    kept[atomicAdd(&sm.count, 1)] = Kept{w, (unsigned)index_of(c), 0u};
+                    atomicAdd(&sm.cut, w);
+                }
+                __syncthreads();
+                const int m = sm.count;
+                const u64 total = sm.cut, target = target_of(total);
+                if (w) {
+                    const unsigned mine = (unsigned)index_of(c);
+                    u64 upto = 0;
+                    for (int j = 0; j < m; ++j) {
+                        const Kept o = kept[j];
+                        upto += o.index <= mine ? o.w : 0;
+                    }
+                    if (upto > target && upto - w <= target) write((int)mine, x, total);
+                }
+                return;
+            }
+        }
+    }
+
+    // ---- the whole row
+    // with an entry of +inf only the entries of +inf have weight (all the same)
+    Row<T, NT, IN_MEMORY, true> again;
+    again.open(logits + (int64_t)r * ld, V);
+    u64 cut = (u64)(best == INFINITY ? kKeyPlusInf : kKeyFinite) << 32;
+    const float reach = fmaxf((float)(S * 0.6931471805599453 * temp), 1e-30f);   // entries further below weigh nothing
+    if (by_k) {
         const u64 k = (u64)top_k;
-        const u64 c = find_cut<false, NT>(row, sm, cut, weight, fmaxf(reach, 1e-30f),
-                                          [&](u64 total) { return k < total ? k : total; });
+        const u64 c = find_cut<false, NT>(again, sm, cut, weight, reach, [&](u64 total) { return k < total ? k : total; });
         cut = c > cut ? c : cut;
     }
-    if (top_p < 1.0)
-        cut = find_cut<true, NT>(row, sm, cut, weight, fmaxf(reach, 1e-30f), [&](u64 total) {
-            const double w = ceil(top_p * (double)total);
-            const u64 want = w < 1.0 ? 1 : (u64)w;
-            return want < total ? want : total;
-        });
-    const unsigned cut_key = (unsigned)(cut >> 32);
+    if (by_p) cut = find_cut<true, NT>(again, sm, cut, weight, reach, prefix_mass);
+    const float cut_x = value_of(cut);
     const unsigned cut_index = ~(unsigned)cut;
-    const double floor_z = min_p > 0.0 ? log(min_p) * temp : -INFINITY;   // w >= min_p as x - top >= T log(min_p)
     auto mass = [&](float x, int i) -> u64 {
-        const unsigned key = order_key(x);
-        if (!(key > cut_key || (key == cut_key && (unsigned)i <= cut_index))) return 0;
+        if (!(x > cut_x || (x == cut_x && (unsigned)i <= cut_index))) return 0;
         if (x != best && (double)x - (double)best < floor_z) return 0;
         return weight(x);
     };
     const u64 total = wave_totals<NT>(row, sm, mass);
-    const double want = u * (double)total;
-    u64 target = want > 0.0 ? (u64)fmin(want, 0x1p63) : 0;
-    if (target >= total) target = total - 1;
-    const int token = locate<NT>(row, sm, target, mass);
-    if (tid == 0) {
-        tokens[r * token_stride] = token;
-        if (log_prob) {
-            const float x = Elem<T>::value(__builtin_bit_cast(typename Elem<T>::Raw, row.src[token]));
-            const double z = x == best ? 0.0 : ((double)x - (double)best) / temp;
-            log_prob[r * lp_stride] = (float)(z - log(ldexp((double)total, -S)));
-        }
-    }
+    const int token = locate<NT>(again, sm, target_of(total), mass);
+    if (tid == 0) write(token, Elem<T>::value(__builtin_bit_cast(typename Elem<T>::Raw, row.src[token])), total);
 }
 
 // ---------------------------------------------------------------------------------------------- top-k and log-normaliser
@@ -393,76 +554,73 @@ __global__ __launch_bounds__(NT) void topk_lse_kernel(const T* __restrict__ logi
     __shared__ Shared<NT> sm;
     __shared__ double sums[NT / 64];
     const int r = blockIdx.x, tid = threadIdx.x;
-    Row<T, NT, PLACE, true> row;
-    extern __shared__ __attribute__((aligned(16))) unsigned char staged[];
-    row.open(logits + (int64_t)r * ld, V, staged);
-    float best = -INFINITY, low = INFINITY;
+    Row<T, NT, PLACE, false> row;
+    row.open(logits + (int64_t)r * ld, V);
+    float best = -INFINITY;
     bool nan = false;
     if (tid == 0) sm.flag = 0;
-    row.each([&](float x, int i) {
+    row.each([&](float x, int) {
         best = fmaxf(best, x);
-        nan |= x != x && i < V;
+        nan |= x != x;
     });
-    low = best;   // the thread's own largest: the k-th largest of the row is no lower than the lowest of k threads'
+    const float own = best;
     best = block_max<NT>(best, sm.red);
     if (nan) sm.flag = 1;
     if (lse) {
-        double s = 0.0;
-        if (best > -INFINITY && best < INFINITY) {
+        const bool some = best > -INFINITY && best < INFINITY;
+        float part = 0.f;
+        if (some) {
             const float c = (float)(per_t * 1.4426950408889634074);
-            float part = 0.f;
-            row.each([&](float x, int) { if (x == x) part += __builtin_amdgcn_exp2f((x - best) * c); });
-            s = part;
+            row.each([&](float x, int) { part += __builtin_amdgcn_exp2f((x - best) * c); });
         }
-        s = wave_sum_d(s);
-        __syncthreads();
+        double s = wave_sum_d((double)part);
         if ((tid & 63) == 0) sums[tid >> 6] = s;
         __syncthreads();
         if (tid == 0) {
             s = 0.0;
             for (int w = 0; w < NT / 64; ++w) s += sums[w];
-            const bool some = best > -INFINITY && best < INFINITY;
             lse[r] = sm.flag ? NAN : some ? (float)((double)best * per_t + log(s)) : best;
         }
     }
-    const float lowest = -block_max<NT>(-low, sm.red);
-    const float width = lowest > -INFINITY && best < INFINITY ? fmaxf((best - lowest) * 1.001f, 1e-30f) : 64.f;
-    const Weights weight{best, 0.0, 0};
-    const u64 want = (u64)k;
-    const u64 cut = find_cut<false, NT>(row, sm, (u64)kKeyNan << 32, weight, width, [&](u64) { return want; });
-    __syncthreads();
-    if (tid == 0) sm.count = 0;
-    __syncthreads();
-    row.each([&](float x, int i) {
-        const u64 c = composite(order_key(x), i);
-        if (c >= cut) sm.hist[atomicAdd(&sm.count, 1)] = c;   // exactly k entries, k <= NT
-    });
-    __syncthreads();
-    u64 c = tid < k ? sm.hist[tid] : 0;
-    c = block_sort<NT>(c, sm.hist);
+    const float bound = k <= NT / 2 ? bound_of<NT>(own, k, sm) : -INFINITY;
+    int n = NT + 1;
+    if (bound > -INFINITY) n = collect<NT>(row, sm, bound, NT);
+    if (n > NT) {   // more ties than threads, a long list, or a row with fewer than k entries above -inf
+        Row<T, NT, IN_MEMORY, true> again;
+        again.open(logits + (int64_t)r * ld, V);
+        const Weights weight{best, 0.0, 0};
+        const float lowest = -block_max<NT>(-own, sm.red);   // the NT-th largest entry is no lower than the lowest thread's
+        const float width = lowest > -INFINITY && best < INFINITY ? fmaxf((best - lowest) * 1.001f, 1e-30f) : 64.f;
+        const u64 want = (u64)k;
+        const u64 cut = find_cut<false, NT>(again, sm, (u64)kKeyNan << 32, weight, width, [&](u64) { return want; });
+        __syncthreads();
+        if (tid == 0) sm.count = 0;
+        __syncthreads();
+        again.each([&](float x, int i) {
+            const u64 c = composite(order_key(x), i);
+            if (c >= cut) sm.hist[atomicAdd(&sm.count, 1)] = c;   // exactly k entries, k <= NT
+        });
+        __syncthreads();
+        n = k;
+    }
+    const u64 c = ranked<NT>(n, sm);
     if (tid < k) {
-        const unsigned key = (unsigned)(c >> 32);
-        const int i = (int)~(unsigned)c;
-        values[(int64_t)r * k + tid] = __uint_as_float(key ^ ((key >> 31) ? 0x80000000u : 0xFFFFFFFFu));
-        indices[(int64_t)r * k + tid] = i;
+        values[(int64_t)r * k + tid] = value_of(c);
+        indices[(int64_t)r * k + tid] = index_of(c);
     }
 }
 
 constexpr int MAX_K = 1024, MAX_V = 1 << 22;
 
-// Workgroup size, and whether the row is staged in LDS, for rows of V entries of which `list` are to be ranked.
-#define ICRL_ROW_DISPATCH(T, V, list, CALL)                                                                       \
-    do {                                                                                                          \
-        constexpr int vec_ = icrl::Elem<T>::VEC;                                                                  \
-        if ((V) <= 256 * 4 * vec_ && (list) <= 256) { CALL(T, 256, IN_LDS); }                                     \
-        else if ((V) <= 512 * 8 * vec_ && (list) <= 512) { CALL(T, 512, IN_LDS); }                                \
-        else { CALL(T, 1024, IN_MEMORY); }                                                                        \
+// Workgroup size and vectors per thread in registers for rows of V entries of which `list` are to be ranked.
+#define ICRL_ROW_DISPATCH(T, V, list, CALL)                                          \
+    do {                                                                             \
+        constexpr int vec_ = icrl::Elem<T>::VEC;                                     \
+        if ((V) <= 256 * 4 * vec_ && (list) <= 256) { CALL(T, 256, 4); }             \
+        else if ((V) <= 512 * 8 * vec_ && (list) <= 512) { CALL(T, 512, 8); }        \
+        else if ((V) <= 1024 * 8 * vec_) { CALL(T, 1024, 8); }                       \
+        else { CALL(T, 1024, IN_MEMORY); }                                           \
     } while (0)
-template <typename T, int NT, int PLACE>
-size_t staged_bytes(int V) {
-    if constexpr (PLACE == IN_LDS) return (size_t)16 * Row<T, NT, PLACE, true>::lds_vectors(V);
-    else return 0;
-}
 }  // namespace
 
 extern "C" int icrl_sample_tokens_filtered(const void* logits, int dtype, int64_t ld_logits, int N, int V,
@@ -483,7 +641,7 @@ extern "C" int icrl_sample_tokens_filtered(const void* logits, int dtype, int64_
     const int S = std::min(51, 62 - bits);
     const Setting t{temperature_rows, temperature}, p{top_p_rows, top_p}, q{min_p_rows, min_p};
 #define ICRL_CALL(T, NT, PLACE)                                                                                           \
-    hipLaunchKernelGGL((sample_filtered_kernel<T, NT, PLACE>), dim3(N), dim3(NT), (staged_bytes<T, NT, PLACE>(V)), icrl::as_stream(stream),             \
+    hipLaunchKernelGGL((sample_filtered_kernel<T, NT, PLACE>), dim3(N), dim3(NT), 0, icrl::as_stream(stream),             \
                        static_cast<const T*>(logits), ld_logits, V, S, uniforms, t, top_k_rows, top_k, p, q, tokens_out, \
                        token_stride, log_prob, log_prob_stride)
     switch (dtype) {
@@ -505,7 +663,7 @@ extern "C" int icrl_topk_lse_rows(const void* logits, int dtype, int64_t ld_logi
     ICRL_REQUIRE(k >= 1 && k <= V && k <= MAX_K, "icrl_topk_lse_rows: k must be in [1, min(%d, V)] (got %d)", MAX_K, k);
     ICRL_REQUIRE(temperature > 0.0 && isfinite(temperature), "icrl_topk_lse_rows: temperature must be positive and finite");
 #define ICRL_CALL(T, NT, PLACE)                                                                                     \
-    hipLaunchKernelGGL((topk_lse_kernel<T, NT, PLACE>), dim3(N), dim3(NT), (staged_bytes<T, NT, PLACE>(V)), icrl::as_stream(stream),              \
+    hipLaunchKernelGGL((topk_lse_kernel<T, NT, PLACE>), dim3(N), dim3(NT), 0, icrl::as_stream(stream),              \
                        static_cast<const T*>(logits), ld_logits, V, k, 1.0 / temperature, values, indices, lse)
     switch (dtype) {
         case ICRL_F32: ICRL_ROW_DISPATCH(float, V, k, ICRL_CALL); break;

@@ -29,9 +29,9 @@ struct Elem<_Float16> {
 };
 
 // Where a row's entries are between the passes over it.  PLACE > 0: in registers, at most PLACE vectors of 16 bytes a
-// thread, for operators with a few short passes (every pass is unrolled).  IN_LDS: staged once.  IN_MEMORY: every pass
-// reads the row again, from the caches where it fits them.
-constexpr int IN_MEMORY = 0, IN_LDS = -1;
+// thread (every pass is unrolled, so passes have to be short).  IN_MEMORY: every pass reads the row again, from the caches
+// where it fits them.
+constexpr int IN_MEMORY = 0;
 
 // A row is cut into one contiguous piece per wave, a multiple of 64 x 16 bytes, and a piece into wave-wide vectors of
 // 16 bytes a lane: reads are 1 KB of consecutive bytes, and (wave, vector, lane, element) is the order of the indices,
@@ -49,13 +49,9 @@ struct Row {
     struct alignas(16) Pack { Raw e[VEC]; };
     typedef unsigned Words __attribute__((ext_vector_type(4), aligned(2), may_alias));   // one 16-byte access
     const T* src;
-    Pack* staged;        // IN_LDS: the workgroup's copy, this thread's first vector
     int V, vectors;      // vectors: how many per thread
     int first;           // index of the thread's first entry
     Pack keep[PLACE > 0 ? PLACE : 1];
-
-    // 16-byte vectors that a workgroup stages for a row of V entries
-    static __host__ __device__ int lds_vectors(int V) { return (V + NT * VEC - 1) / (NT * VEC) * NT; }
 
     __device__ __forceinline__ Pack read(int i) const {
         const int at = first + i * 64 * VEC;
@@ -84,33 +80,18 @@ struct Row {
         return p;
     }
     __device__ __forceinline__ Pack fetch(int i) const {
-        if constexpr (PLACE == IN_LDS) return staged[i * 64];
-        else return canonical(read(i), i);
+        return canonical(read(i), i);
     }
 
-    // lds: lds_vectors(count) vectors if IN_LDS.  No barrier is needed: a thread reads back what it wrote itself.
-    __device__ __forceinline__ void open(const T* row, int count, void* lds) {
+    __device__ __forceinline__ void open(const T* row, int count) {
         src = row;
         V = count;
         vectors = (count + NT * VEC - 1) / (NT * VEC);
-        const int at = (int)(threadIdx.x >> 6) * vectors * 64 + (int)(threadIdx.x & 63);
-        first = at * VEC;
-        staged = static_cast<Pack*>(lds) + at;
+        first = ((int)(threadIdx.x >> 6) * vectors * 64 + (int)(threadIdx.x & 63)) * VEC;
         if constexpr (PLACE > 0) {
 #pragma unroll
             for (int i = 0; i < PLACE; ++i)
                 if (i < vectors) keep[i] = canonical(read(i), i);
-        } else if constexpr (PLACE == IN_LDS) {
-            constexpr int AHEAD = 4;   // reads in flight per thread
-            for (int i = 0; i < vectors; i += AHEAD) {
-                Pack p[AHEAD];
-#pragma unroll
-                for (int q = 0; q < AHEAD; ++q)
-                    if (i + q < vectors) p[q] = read(i + q);
-#pragma unroll
-                for (int q = 0; q < AHEAD; ++q)
-                    if (i + q < vectors) staged[(i + q) * 64] = canonical(p[q], i + q);
-            }
         }
     }
 
@@ -121,8 +102,6 @@ struct Row {
 #pragma unroll
             for (int i = 0; i < PLACE; ++i)
                 if (i < vectors) f(keep[i], first + i * 64 * VEC);
-        } else if constexpr (PLACE == IN_LDS) {
-            for (int i = 0; i < vectors; ++i) f(staged[i * 64], first + i * 64 * VEC);
         } else {
             constexpr int AHEAD = 4;
             for (int i = 0; i < vectors; i += AHEAD) {
