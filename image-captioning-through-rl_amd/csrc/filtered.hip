@@ -9,10 +9,10 @@
 // on lists of at most a thread per entry:
 //   - The k-th largest of the threads' own maxima is a lower bound of the k-th largest entry, and hardly more than k
 //     entries reach it.  They are collected and ranked; filters that start from a top-k never look at the row again.
-//   - min-p alone is a bound itself.  top-p alone needs the whole row's mass, then tries the same short list.
-//   - Where the list does not reach (a flat distribution's nucleus, or more ties than threads), a histogram over 2048
-//     value ranges names the range that the cut falls into, and only that range is ranked, or refined by radix passes
-//     over its keys when even it is too long.
+//   - min-p is a bound itself.
+//   - top-p alone: a histogram of the masses of 2048 value ranges names the range that the cut falls into, and only that
+//     range is ranked.  Where a list gets longer than the threads (ties), or top-k is large, the same is done with exact
+//     sums, and a range that is too long even so is refined by radix passes over its keys.
 //
 // Masses are 64-bit integers, multiples of 2^-S of the row's largest weight with S = 62 - ceil(log2 V) (at most 51):
 // integer sums have no order, so atomics and any split of the row give the same bits, and 2^-45 of the largest weight
@@ -47,18 +47,23 @@ __device__ __forceinline__ float value_of(u64 c) {
 }
 __device__ __forceinline__ int index_of(u64 c) { return (int)~(unsigned)c; }
 
-// Weights of one row: e^((x - top) / T) as multiples of 2^-S.
+// Weights of one row: e^((x - top) / T) as multiples of 2^-S.  An infinite top counts as the largest finite number (as do
+// the entries equal to it; the callers see to it that no others are kept then).
 struct Weights {
-    float top;
-    double per_unit;   // log2(e) / T
+    double top, per_unit;   // per_unit = log2(e) / T
     int S;
-    __device__ __forceinline__ u64 operator()(float x) const {
-        const double t = x == top ? 0.0 : ((double)x - (double)top) * per_unit;
-        if (!(t > -(double)(S + 2))) return 0;
-        const double one = ldexp(exp2_neg(t), S);             // at most 2^51
-        return (u64)(__double_as_longlong(one + 0x1p52) & 0xFFFFFFFFFFFFFll);   // the sum's low 52 bits: `one` to the nearest integer
+    __device__ __forceinline__ double units(float x) const {   // before rounding
+        const double t = ((double)fminf(x, 3.402823466e38f) - top) * per_unit;
+        return exp2_scaled(fmax(t, -(double)(S + 2)), S);       // at least 1/4, which rounds to nothing; at most 2^51
     }
+    static __device__ __forceinline__ u64 rounded(double units) {   // the sum's low 52 bits: units to the nearest integer
+        return (u64)__double_as_longlong(units + 0x1p52) & ((1ull << 52) - 1);
+    }
+    __device__ __forceinline__ u64 operator()(float x) const { return rounded(units(x)); }
 };
+__device__ __forceinline__ Weights weights_of(float best, double temp, int S) {
+    return Weights{(double)fminf(best, 3.402823466e38f), 1.4426950408889634074 / temp, S};
+}
 
 template <int NT>
 __device__ __forceinline__ float block_max(float v, float* red) {
@@ -178,15 +183,15 @@ __device__ __forceinline__ int locate(const R& row, Shared<NT>& sm, u64 target, 
     return sm.index;
 }
 
-// Where the running sum of sm.hist (bin 0 first) reaches `need` (which need_of makes from the total): bin in sm.bin, the
+// Where the running sum of the bins (bin_at(0) first) reaches `need` (which need_of makes from the total): bin in sm.bin, the
 // sum of the bins before it in sm.above.  Returns need.
-template <int NT, typename G>
-__device__ __forceinline__ u64 find_bin(Shared<NT>& sm, G&& need_of) {
+template <int NT, typename H, typename G>
+__device__ __forceinline__ u64 find_bin(Shared<NT>& sm, H&& bin_at, G&& need_of) {
     constexpr int PER = BINS / NT;
     u64 own[PER], sum = 0;
 #pragma unroll
     for (int b = 0; b < PER; ++b) {
-        own[b] = sm.hist[threadIdx.x * PER + b];
+        own[b] = bin_at(threadIdx.x * PER + b);
         sum += own[b];
     }
     u64 run = block_prefix<NT>(sum, sm);
@@ -210,57 +215,117 @@ __device__ __forceinline__ void clear_hist(Shared<NT>& sm) {
     __syncthreads();
 }
 
+// Sorts the n <= NT composites in sm.hist: thread i gets the i-th of the order (0 past the end).  Short lists are ranked
+// by comparing all with all (n / 2 reads of two entries each, 0.5 us at n = 100 against 2.8 us for the sort).
+template <int NT>
+__device__ __forceinline__ u64 ranked(int n, Shared<NT>& sm) {
+    const int tid = threadIdx.x;
+    if (n <= 256 && n < BINS / 2) {
+        u64* out = sm.hist + BINS / 2;
+        if (tid == 0) sm.hist[n] = 0;   // an even number of entries to read
+        __syncthreads();
+        if (tid < n) {
+            const u64 mine = sm.hist[tid];
+            const ulonglong2* two = reinterpret_cast<const ulonglong2*>(sm.hist);
+            int rank = 0;
+            for (int j = 0; j < (n + 1) / 2; ++j) {
+                const ulonglong2 o = two[j];
+                rank += (o.x > mine) + (o.y > mine);
+            }
+            out[rank] = mine;
+        }
+        __syncthreads();
+        return tid < n ? out[tid] : 0;
+    }
+    const u64 c = tid < n ? sm.hist[tid] : 0;
+    return block_sort<NT>(c, sm.hist);
+}
+
 // The cut after the shortest prefix (in the row's order, among the entries with composite >= `from`) whose amounts -
-// MASS: weights, else 1 each - reach need_of(total).  width: the value range that the first histogram spreads over its
+// by_mass: weights, else 1 each - reach need_of(total).  width: the value range that the first histogram spreads over its
 // bins, counted from the top; any positive width gives the same cut, a good one makes the second step short.
-template <bool MASS, int NT, typename R, typename G>
-__device__ __forceinline__ u64 find_cut(const R& row, Shared<NT>& sm, u64 from, const Weights& weight, float width, G&& need_of) {
-    const unsigned from_key = (unsigned)(from >> 32);
-    const unsigned from_index = ~(unsigned)from;
+// Weights are computed for a whole vector before anything depends on one of them: a weight is a chain of some 20 float64
+// instructions, and only side by side do they hide each other's latency (400 clocks an entry otherwise, 100 so).
+// Returns with the kept masses of the waves' pieces in sm.part and their total in `mass_kept` if by_mass and the second
+// step was the short one; otherwise mass_kept is 0.
+template <int NT, typename R, typename G>
+__device__ __forceinline__ u64 find_cut(const R& row, Shared<NT>& sm, bool by_mass, u64 from, const Weights& weight, float width,
+                                        G&& need_of, u64& mass_kept) {
+    constexpr int VEC = R::VEC;
+    const unsigned from_key = (unsigned)(from >> 32), from_index = ~(unsigned)from;
     auto kept = [&](unsigned key, int i) { return key > from_key || (key == from_key && (unsigned)i <= from_index); };
-    auto amount = [&](float x) { return MASS ? weight(x) : (u64)1; };
-    const float per = (float)BINS / width, top = weight.top;
+    auto amount = [&](float x) { return by_mass ? weight(x) : (u64)1; };
+    const float per = (float)BINS / width, top = (float)weight.top;
     auto bin = [&](float x) {   // monotone in the row's order; what is far below the top, NaN included, is the last bin
         const float at = (top - x) * per;
-        return at < (float)(BINS - 1) ? (int)at : BINS - 1;
+        return at < (float)(BINS - 1) ? (int)fmaxf(at, 0.f) : BINS - 1;   // (+inf lies above a finite top: bin 0)
     };
+    auto amounts = [&](const typename R::Pack& p, u64 (&a)[VEC]) {
+        if (by_mass) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) a[j] = weight(Elem<typename R::Type>::value(p.e[j]));
+        } else {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) a[j] = 1;
+        }
+    };
+    mass_kept = 0;
     clear_hist<NT>(sm);
     if (threadIdx.x == 0) { sm.count = 0; sm.key_lo = ~0u; sm.key_hi = 0; }
     u64 rest = 0;   // the last bin, which may hold most of the row, is summed in registers
-    row.each([&](float x, int i) {
-        if (kept(order_key(x), i)) {
-            const u64 a = amount(x);
+    row.each_pack([&](const typename R::Pack& p, int at) {
+        u64 a[VEC];
+        amounts(p, a);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            const float x = Elem<typename R::Type>::value(p.e[j]);
             const int b = bin(x);
-            if (b == BINS - 1) rest += a;
-            else if (a) atomicAdd(&sm.hist[b], a);
+            const bool in = kept(order_key(x), at + j);
+            rest += in && b == BINS - 1 ? a[j] : 0;
+            if (in && b < BINS - 1) atomicAdd(&sm.hist[b], a[j]);
         }
     });
     rest = wave_sum_u64(rest);
     if ((threadIdx.x & 63) == 0 && rest) atomicAdd(&sm.hist[BINS - 1], rest);
     __syncthreads();
-    u64 need = find_bin<NT>(sm, need_of);
+    auto counted = [&](int b) { return sm.hist[b]; };
+    u64 need = find_bin<NT>(sm, counted, need_of);
     const int b0 = sm.bin;
-    need -= sm.above;
+    const u64 above = sm.above;
+    need -= above;
     __syncthreads();   // the histogram's place now takes the entries of that bin
-    row.each([&](float x, int i) {
-        const unsigned key = order_key(x);
-        if (kept(key, i) && bin(x) == b0) {
-            const int at = atomicAdd(&sm.count, 1);
-            if (at < NT) sm.hist[at] = composite(key, i);
+    u64 sure = 0;      // this thread's share of the mass above it
+    row.each_pack([&](const typename R::Pack& p, int at) {
+        u64 a[VEC];
+        amounts(p, a);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            const float x = Elem<typename R::Type>::value(p.e[j]);
+            const int b = bin(x);
+            const bool in = kept(order_key(x), at + j);
+            sure += in && b < b0 ? a[j] : 0;
+            if (in && b == b0) {
+                const int to = atomicAdd(&sm.count, 1);
+                if (to < NT) sm.hist[to] = composite(order_key(x), at + j);
+            }
         }
     });
+    sure = wave_sum_u64(sure);
     __syncthreads();
     const int members = sm.count;
     if (members <= NT) {
-        u64 c = (int)threadIdx.x < members ? sm.hist[threadIdx.x] : 0;
-        c = block_sort<NT>(c, sm.hist);
-        u64 a = 0;
-        if (c != 0) {
-            a = amount(value_of(c));
-        }
+        const u64 c = ranked<NT>(members, sm);
+        const u64 a = c ? amount(value_of(c)) : 0;
         const u64 before = block_prefix<NT>(a, sm);
-        if (before < need && before + a >= need) sm.cut = c;
         __syncthreads();
+        if ((threadIdx.x & 63) == 0) sm.part[threadIdx.x >> 6] = sure;
+        if (before < need && before + a >= need) { sm.cut = c; sm.total = before + a; }
+        __syncthreads();
+        if (by_mass) {
+            mass_kept = above + sm.total;
+            if (a && before < need) atomicAdd(&sm.part[index_of(c) / (row.vectors * 64 * VEC)], a);
+            __syncthreads();
+        }
         return sm.cut;
     }
     // many entries in one range: radix over the keys that occur in it, 11 bits a pass
@@ -286,7 +351,7 @@ __device__ __forceinline__ u64 find_cut(const R& row, Shared<NT>& sm, u64 from, 
         });
         __syncthreads();
         const u64 want = need;
-        find_bin<NT>(sm, [&](u64) { return want; });
+        find_bin<NT>(sm, counted, [&](u64) { return want; });
         need -= sm.above;
         const unsigned upper = hi - ((unsigned)sm.bin << shift);
         const unsigned span = (1u << shift) - 1u;
@@ -310,7 +375,7 @@ template <int NT>
 __device__ __forceinline__ float bound_of(float own_max, int k, Shared<NT>& sm) {
     unsigned* keys = reinterpret_cast<unsigned*>(sm.hist);
     __syncthreads();
-    keys[threadIdx.x] = order_key(own_max + 0.f);
+    keys[threadIdx.x] = order_key(own_max);
     __syncthreads();
     if (threadIdx.x < 64) {
         unsigned key[NT / 64], t = 0;
@@ -340,43 +405,18 @@ __device__ __forceinline__ int collect(const R& row, Shared<NT>& sm, float bound
     __syncthreads();
     row.each_pack([&](const typename R::Pack& p, int at) {
         float most = -INFINITY;
-        row.vector(p, at, [&](float x, int) { most = fmaxf(most, x); });
-        if (most >= bound)
-            row.vector(p, at, [&](float x, int i) {
-                if (x >= bound) {
-                    const int to = atomicAdd(&sm.count, 1);
-                    if (to < room) sm.hist[to] = composite(order_key(x + 0.f), i);
-                }
-            });
+#pragma unroll
+        for (int j = 0; j < R::VEC; ++j) most = fmaxf(most, Elem<typename R::Type>::value(p.e[j]));
+        if (!(most >= bound)) return;
+        row.vector(p, at, [&](float x, int i) {
+            if (x >= bound) {
+                const int to = atomicAdd(&sm.count, 1);
+                if (to < room) sm.hist[to] = composite(order_key(x), i);
+            }
+        });
     });
     __syncthreads();
     return sm.count;
-}
-
-// Sorts the n <= NT composites in sm.hist: thread i gets the i-th of the order (0 past the end).  Short lists are ranked
-// by comparing all with all (n / 2 reads of two entries each, 0.5 us at n = 100 against 2.8 us for the sort).
-template <int NT>
-__device__ __forceinline__ u64 ranked(int n, Shared<NT>& sm) {
-    const int tid = threadIdx.x;
-    if (n <= 256 && n < BINS / 2) {
-        u64* out = sm.hist + BINS / 2;
-        if (tid == 0) sm.hist[n] = 0;   // an even number of entries to read
-        __syncthreads();
-        if (tid < n) {
-            const u64 mine = sm.hist[tid];
-            const ulonglong2* two = reinterpret_cast<const ulonglong2*>(sm.hist);
-            int rank = 0;
-            for (int j = 0; j < (n + 1) / 2; ++j) {
-                const ulonglong2 o = two[j];
-                rank += (o.x > mine) + (o.y > mine);
-            }
-            out[rank] = mine;
-        }
-        __syncthreads();
-        return tid < n ? out[tid] : 0;
-    }
-    const u64 c = tid < n ? sm.hist[tid] : 0;
-    return block_sort<NT>(c, sm.hist);
 }
 
 // ---------------------------------------------------------------------------------------------- sampling
@@ -390,8 +430,8 @@ struct Setting {   // one filter setting: a value for each row, or one for all o
 // those that come no later in the vocabulary; the one whose sum first exceeds the target is drawn.
 struct Kept { u64 w; unsigned index, pad; };
 
-template <typename T, int NT, int PLACE>
-__global__ __launch_bounds__(NT) void sample_filtered_kernel(const T* __restrict__ logits, int64_t ld, int V, int S,
+template <typename T, int NT>
+__global__ __launch_bounds__(NT, 4) void sample_filtered_kernel(const T* __restrict__ logits, int64_t ld, int V, int S,
                                                              const double* __restrict__ uniforms, Setting temperature,
                                                              const int* __restrict__ top_k_rows, int top_k_all,
                                                              Setting top_p_in, Setting min_p_in,
@@ -399,7 +439,9 @@ __global__ __launch_bounds__(NT) void sample_filtered_kernel(const T* __restrict
                                                              float* __restrict__ log_prob, int64_t lp_stride) {
     __shared__ Shared<NT> sm;
     const int r = blockIdx.x, tid = threadIdx.x;
-    Row<T, NT, PLACE, false> row;
+    // Read again by every pass: the passes that weigh entries, unrolled over a row in registers, would be far longer than
+    // the instruction cache, and with registers to spare two workgroups fit a CU (512 rows of 10 000: 33 against 36 us)
+    Row<T, NT, IN_MEMORY, false> row;
     row.open(logits + (int64_t)r * ld, V);
     const double temp = temperature.at(r), top_p = top_p_in.at(r), min_p = min_p_in.at(r), u = uniforms[r];
     const int top_k = top_k_rows ? top_k_rows[r] : top_k_all;
@@ -438,7 +480,7 @@ __global__ __launch_bounds__(NT) void sample_filtered_kernel(const T* __restrict
         }
         return;
     }
-    const Weights weight{best, 1.4426950408889634074 / temp, S};
+    const Weights weight = weights_of(best, temp, S);
     const double floor_z = min_p > 0.0 ? log(min_p) * temp : -INFINITY;   // w >= min_p as x - best >= T log(min_p)
     auto write = [&](int token, float x, u64 total) {
         tokens[r * token_stride] = token;
@@ -462,93 +504,85 @@ __global__ __launch_bounds__(NT) void sample_filtered_kernel(const T* __restrict
     // ---- the short list: entries no smaller than a bound that everything kept reaches
     constexpr int LIST = NT / 2;   // longest list drawn from
     float bound = -INFINITY;
-    bool guess = false;            // whether the bound is only likely to reach far enough
     if (by_k) {
         if (top_k <= NT / 4) bound = bound_of<NT>(own, top_k, sm);
-    } else if (min_p > 0.0) {
+    } else if (min_p > 0.0 && best < INFINITY) {
         const double z = (double)best + floor_z;
         bound = (float)z;
         if ((double)bound > z) bound = nextafterf(bound, -INFINITY);
-        if (best == INFINITY) bound = INFINITY;
-    } else if (by_p) {
-        bound = bound_of<NT>(own, NT / 8, sm);
-        guess = true;
     }
-    u64 row_mass = 0;   // of the whole row, where top_p counts from it
     if (bound > -INFINITY) {
         const int n = collect<NT>(row, sm, bound, LIST);
         if (n <= LIST) {
-            bool whole = true;
             u64 c = 0;
             if (by_k || by_p) c = ranked<NT>(n, sm);
             else if (tid < n) c = sm.hist[tid];
             if (by_k && tid >= top_k) c = 0;
             const float x = c ? value_of(c) : 0.f;
-            u64 w = c ? weight(x) : 0;
+            u64 w = c && (best < INFINITY || x == best) ? weight(x) : 0;
             if (by_p) {
                 const u64 before = block_prefix<NT>(w, sm);
                 const u64 listed = sm.total;
-                if (!by_k) row_mass = wave_totals<NT>(row, sm, [&](float y, int) { return weight(y); });
-                const u64 want = prefix_mass(by_k ? listed : row_mass);
-                whole = listed >= want || !guess;
-                if (before >= want) w = 0;
+                const u64 from = by_k ? listed : wave_totals<NT>(row, sm, [&](float y, int) { return weight(y); });
+                if (before >= prefix_mass(from)) w = 0;
             }
-            if (whole) {
-                if (c && x != best && (double)x - (double)best < floor_z) w = 0;
-                // kept entries side by side, then everyone against everyone
-                Kept* kept = reinterpret_cast<Kept*>(sm.hist);
-                static_assert(sizeof(Kept) * LIST <= sizeof(sm.hist), "the kept list fits the histogram's place");
-                __syncthreads();
-                if (tid == 0) { sm.count = 0; sm.cut = 0; }
-                __syncthreads();
-                if (w) {
-                    kept[atomicAdd(&sm.count, 1)] = Kept{w, (unsigned)index_of(c), 0u};
-                    atomicAdd(&sm.cut, w);
-                }
-                __syncthreads();
-                const int m = sm.count;
-                const u64 total = sm.cut, target = target_of(total);
-                if (w) {
-                    const unsigned mine = (unsigned)index_of(c);
-                    u64 upto = 0;
-                    for (int j = 0; j < m; ++j) {
-                        const Kept o = kept[j];
-                        upto += o.index <= mine ? o.w : 0;
-                    }
-                    if (upto > target && upto - w <= target) write((int)mine, x, total);
-                }
-                return;
+            if (c && x != best && (double)x - (double)best < floor_z) w = 0;
+            // kept entries side by side, then everyone against everyone
+            Kept* kept = reinterpret_cast<Kept*>(sm.hist);
+            static_assert(sizeof(Kept) * LIST <= sizeof(sm.hist), "the kept list fits the histogram's place");
+            __syncthreads();
+            if (tid == 0) { sm.count = 0; sm.cut = 0; }
+            __syncthreads();
+            if (w) {
+                kept[atomicAdd(&sm.count, 1)] = Kept{w, (unsigned)index_of(c), 0u};
+                atomicAdd(&sm.cut, w);
             }
+            __syncthreads();
+            const int m = sm.count;
+            const u64 total = sm.cut, target = target_of(total);
+            if (w) {
+                const unsigned mine = (unsigned)index_of(c);
+                u64 upto = 0;
+                for (int j = 0; j < m; ++j) {
+                    const Kept o = kept[j];
+                    upto += o.index <= mine ? o.w : 0;
+                }
+                if (upto > target && upto - w <= target) write((int)mine, x, total);
+            }
+            return;
         }
     }
 
+    const float reach = fmaxf((float)(S * 0.6931471805599453 * temp), 1e-30f);   // entries further below weigh nothing
+    float cut_x = -INFINITY;
+    unsigned cut_index = 0;
+    auto mass = [&](float x, int i) -> u64 {
+        const u64 w = weight(x);
+        const bool in = (x > cut_x) | ((x == cut_x) & ((unsigned)i <= cut_index));
+        const bool low = (x != best) & ((double)x - (double)best < floor_z);
+        return in & !low ? w : 0;
+    };
+
     // ---- the whole row
     // with an entry of +inf only the entries of +inf have weight (all the same)
-    Row<T, NT, IN_MEMORY, true> again;
-    again.open(logits + (int64_t)r * ld, V);
-    u64 cut = (u64)(best == INFINITY ? kKeyPlusInf : kKeyFinite) << 32;
-    const float reach = fmaxf((float)(S * 0.6931471805599453 * temp), 1e-30f);   // entries further below weigh nothing
-    if (by_k) {
+    u64 cut = (u64)(best == INFINITY ? kKeyPlusInf : kKeyFinite) << 32, total = 0;
+    for (int filter = 0; filter < 2; ++filter) {   // top-k, then top-p: one copy of the code
+        const bool by_mass = filter == 1;
+        if (!(by_mass ? by_p : by_k)) continue;
         const u64 k = (u64)top_k;
-        const u64 c = find_cut<false, NT>(again, sm, cut, weight, reach, [&](u64 total) { return k < total ? k : total; });
-        cut = c > cut ? c : cut;
+        cut = find_cut<NT>(row, sm, by_mass, cut, weight, reach, [&](u64 of) { return by_mass ? prefix_mass(of) : k < of ? k : of; },
+                           total);
     }
-    if (by_p) cut = find_cut<true, NT>(again, sm, cut, weight, reach, prefix_mass);
-    const float cut_x = value_of(cut);
-    const unsigned cut_index = ~(unsigned)cut;
-    auto mass = [&](float x, int i) -> u64 {
-        if (!(x > cut_x || (x == cut_x && (unsigned)i <= cut_index))) return 0;
-        if (x != best && (double)x - (double)best < floor_z) return 0;
-        return weight(x);
-    };
-    const u64 total = wave_totals<NT>(row, sm, mass);
-    const int token = locate<NT>(again, sm, target_of(total), mass);
-    if (tid == 0) write(token, Elem<T>::value(__builtin_bit_cast(typename Elem<T>::Raw, row.src[token])), total);
+    cut_x = value_of(cut);
+    cut_index = ~(unsigned)cut;
+    if (total == 0 || min_p > 0.0) total = wave_totals<NT>(row, sm, mass);
+    const int token = locate<NT>(row, sm, target_of(total), mass);
+    if (tid == 0) write(token, row.entry(token), total);
 }
 
 // ---------------------------------------------------------------------------------------------- top-k and log-normaliser
 template <typename T, int NT, int PLACE>
-__global__ __launch_bounds__(NT) void topk_lse_kernel(const T* __restrict__ logits, int64_t ld, int V, int k, double per_t,
+__global__ __launch_bounds__(NT, 8) void topk_lse_kernel(const T* __restrict__ logits, int64_t ld, int V, int k, double per_t,
                                                       float* __restrict__ values, int64_t* __restrict__ indices,
                                                       float* __restrict__ lse) {
     __shared__ Shared<NT> sm;
@@ -588,11 +622,12 @@ __global__ __launch_bounds__(NT) void topk_lse_kernel(const T* __restrict__ logi
     if (n > NT) {   // more ties than threads, a long list, or a row with fewer than k entries above -inf
         Row<T, NT, IN_MEMORY, true> again;
         again.open(logits + (int64_t)r * ld, V);
-        const Weights weight{best, 0.0, 0};
+        const Weights weight = weights_of(best, INFINITY, 0);   // its top alone is used
         const float lowest = -block_max<NT>(-own, sm.red);   // the NT-th largest entry is no lower than the lowest thread's
         const float width = lowest > -INFINITY && best < INFINITY ? fmaxf((best - lowest) * 1.001f, 1e-30f) : 64.f;
         const u64 want = (u64)k;
-        const u64 cut = find_cut<false, NT>(again, sm, (u64)kKeyNan << 32, weight, width, [&](u64) { return want; });
+        u64 none;
+        const u64 cut = find_cut<NT>(again, sm, false, (u64)kKeyNan << 32, weight, width, [&](u64) { return want; }, none);
         __syncthreads();
         if (tid == 0) sm.count = 0;
         __syncthreads();
@@ -641,7 +676,7 @@ extern "C" int icrl_sample_tokens_filtered(const void* logits, int dtype, int64_
     const int S = std::min(51, 62 - bits);
     const Setting t{temperature_rows, temperature}, p{top_p_rows, top_p}, q{min_p_rows, min_p};
 #define ICRL_CALL(T, NT, PLACE)                                                                                           \
-    hipLaunchKernelGGL((sample_filtered_kernel<T, NT, PLACE>), dim3(N), dim3(NT), 0, icrl::as_stream(stream),             \
+    hipLaunchKernelGGL((sample_filtered_kernel<T, NT>), dim3(N), dim3(NT), 0, icrl::as_stream(stream),             \
                        static_cast<const T*>(logits), ld_logits, V, S, uniforms, t, top_k_rows, top_k, p, q, tokens_out, \
                        token_stride, log_prob, log_prob_stride)
     switch (dtype) {

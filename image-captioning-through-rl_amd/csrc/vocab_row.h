@@ -40,11 +40,11 @@ constexpr int IN_MEMORY = 0;
 // the canonical NaN included; CANON also turns every NaN into one and -0 into +0, so that equal entries have equal keys.
 template <typename T, int NT, int PLACE, bool CANON>
 struct Row {
-    static constexpr int VEC = Elem<T>::VEC, NW = NT / 64;
+    using Type = T;
+    static constexpr int VEC = Elem<T>::VEC;
     using Raw = typename Elem<T>::Raw;
     static constexpr Raw kNan = sizeof(T) == 4 ? (Raw)0xFFC00000u : (__is_same(T, __bf16) ? (Raw)0xFFC0u : (Raw)0xFE00u);
     static constexpr Raw kMinusInf = sizeof(T) == 4 ? (Raw)0xFF800000u : (__is_same(T, __bf16) ? (Raw)0xFF80u : (Raw)0xFC00u);
-    static constexpr Raw kMinusZero = (Raw)((Raw)1 << (8 * sizeof(Raw) - 1));
     static constexpr Raw kFill = CANON ? (Raw)~0u : kMinusInf;
     struct alignas(16) Pack { Raw e[VEC]; };
     typedef unsigned Words __attribute__((ext_vector_type(4), aligned(2), may_alias));   // one 16-byte access
@@ -73,8 +73,7 @@ struct Row {
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
                 const float x = Elem<T>::value(p.e[j]);
-                const Raw same = p.e[j] == kMinusZero ? (Raw)0 : p.e[j];
-                p.e[j] = x != x && at + j < V ? kNan : same;
+                p.e[j] = x != x && at + j < V ? kNan : p.e[j];
             }
         }
         return p;
@@ -95,13 +94,25 @@ struct Row {
         }
     }
 
+    // A vector as a pass sees it.  16-bit entries are widened anew in every pass: the compiler, which would otherwise widen
+    // the row once for all of them and then has twice its registers to keep, is told that they may have changed.
+    static __device__ __forceinline__ Pack pass(const Pack& p) {
+        Words w = __builtin_bit_cast(Words, p);
+        if (sizeof(T) == 2) asm("" : "+v"(w));
+        return __builtin_bit_cast(Pack, w);
+    }
+    // entry i < V, from memory
+    __device__ __forceinline__ float entry(int i) const {
+        const float x = Elem<T>::value(__builtin_bit_cast(Raw, src[i]));
+        return CANON && x != x ? Elem<T>::value(kNan) : x;
+    }
     // f(vector, index of its first entry) for each of the thread's vectors
     template <typename F>
     __device__ __forceinline__ void each_pack(F&& f) const {
         if constexpr (PLACE > 0) {
 #pragma unroll
             for (int i = 0; i < PLACE; ++i)
-                if (i < vectors) f(keep[i], first + i * 64 * VEC);
+                if (i < vectors) f(pass(keep[i]), first + i * 64 * VEC);
         } else {
             constexpr int AHEAD = 4;
             for (int i = 0; i < vectors; i += AHEAD) {
@@ -133,29 +144,27 @@ struct Row {
 // Unsigned keys in the order of the values.  -inf: 0x007FFFFF; the canonical NaN below it, places past the end below that.
 constexpr unsigned kKeyNan = 0x003FFFFFu, kKeyMinusInf = 0x007FFFFFu, kKeyFinite = 0x00800000u, kKeyPlusInf = 0xFF800000u;
 __device__ __forceinline__ unsigned order_key(float x) {
-    const int b = __float_as_int(x);
+    int b = __float_as_int(x);
+    b = b == (int)0x80000000 ? 0 : b;   // -0 and +0 are equal
     return (unsigned)(b ^ ((b >> 31) | (int)0x80000000));
 }
 
-// 2^t for t <= 0 in float64, by the Taylor series of 2^r = e^(r ln 2) on |r| <= 1/2: eleven terms leave
-// 0.3466^12 / 12! = 6e-15.  (The library's exp2 spends several times the instructions on the last two bits.)
-__device__ __forceinline__ double exp2_neg(double t) {
+// 2^t 2^scale in float64, by the Taylor series of 2^r = e^(r ln 2) on |r| <= 1/2: nine terms leave 0.3466^10 / 10! =
+// 7e-12 of the result.  (The library's exp2 spends several times the instructions on bits that no sum here can show.)
+__device__ __forceinline__ double exp2_scaled(double t, int scale) {
     const double n = rint(t), r = t - n;
-    constexpr double L = 0.69314718055994530942;
-    double p = 1.0 / 39916800.0;
-    const double y = r * L;
-    p = fma(p, y, 1.0 / 3628800.0);
-    p = fma(p, y, 1.0 / 362880.0);
-    p = fma(p, y, 1.0 / 40320.0);
-    p = fma(p, y, 1.0 / 5040.0);
-    p = fma(p, y, 1.0 / 720.0);
-    p = fma(p, y, 1.0 / 120.0);
-    p = fma(p, y, 1.0 / 24.0);
-    p = fma(p, y, 1.0 / 6.0);
-    p = fma(p, y, 0.5);
-    p = fma(p, y, 1.0);
-    p = fma(p, y, 1.0);
-    return ldexp(p, (int)n);
+    constexpr double L = 0.69314718055994530942, L2 = L * L, L3 = L2 * L, L4 = L2 * L2, L5 = L4 * L;
+    double p = L4 * L5 / 362880.0;
+    p = fma(p, r, L4 * L4 / 40320.0);
+    p = fma(p, r, L4 * L3 / 5040.0);
+    p = fma(p, r, L3 * L3 / 720.0);
+    p = fma(p, r, L5 / 120.0);
+    p = fma(p, r, L4 / 24.0);
+    p = fma(p, r, L3 / 6.0);
+    p = fma(p, r, L2 / 2.0);
+    p = fma(p, r, L);
+    p = fma(p, r, 1.0);
+    return ldexp(p, (int)n + scale);
 }
 
 __device__ __forceinline__ u64 wave_sum_u64(u64 v) {
