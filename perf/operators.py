@@ -18,9 +18,16 @@ BYTES = {"f32": 4, "bf16": 2, "f16": 2}
 BLOCK = 128   # entries that share a scale in an 8-bit operand
 
 
+_bindings = None
+
+
 def _hip():
-    import importlib
-    return importlib.import_module("image-captioning-through-rl_amd.hipabi")
+    """This repository's bindings, imported once."""
+    global _bindings
+    if _bindings is None:
+        import importlib
+        _bindings = importlib.import_module("image-captioning-through-rl_amd.hipabi")
+    return _bindings
 
 
 def listed():
