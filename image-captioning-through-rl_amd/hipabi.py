@@ -250,37 +250,36 @@ def _chain_shapes(who, n, p0, n_calls, gates, xproj=None, h_emit=None, saved=Non
 
 
 def _dtype_code(t):
-    assert t.dtype in DTYPES, "float32, bfloat16 or float16 expected, got %s" % t.dtype
-    return DTYPES[t.dtype]
+    code = DTYPES.get(t.dtype)
+    assert code is not None, "float32, bfloat16 or float16 expected, got %s" % t.dtype
+    return code
 
 
 def _row_stride(t):
-    """Row stride of a 2-D tensor whose rows are contiguous (of a single row, or a single column: any that is valid)."""
-    assert t.dim() == 2 and (t.stride(1) == 1 or t.shape[1] == 1), "rows must be contiguous"
-    return t.stride(0) if t.shape[0] > 1 and t.stride(0) >= t.shape[1] else _no_overlap(t)
+    """Row stride of a 2-D tensor whose rows are contiguous and do not overlap (of a single row: its length)."""
+    rows, width = t.shape
+    step, unit = t.stride()
+    assert unit == 1 or width == 1, "rows must be contiguous"
+    assert step >= width or rows <= 1, "rows must not overlap"
+    return step if step >= width else width
 
 
-def _no_overlap(t):
-    assert t.shape[0] <= 1, "rows must not overlap"
-    return t.shape[1]
-
-
-def _on_current_device(*tensors):
-    """Launches go to the current device's stream: every operand must live there."""
-    current = None
-    for t in tensors:
-        if isinstance(t, torch.Tensor):
-            assert t.is_cuda, "the HIP kernels take device tensors"
-            if current is None:
-                current = torch.cuda.current_device() if _raw_device is None else _raw_device()
-            assert t.get_device() == current, "operand on cuda:%d, the current device is cuda:%d" % (t.get_device(), current)
+def _on_current_device(first, *others):
+    """Launches go to the current device's stream: every operand (None: absent) must live there."""
+    d = first.get_device()
+    assert d >= 0, "the HIP kernels take device tensors"
+    for t in others:
+        assert t is None or t.get_device() == d, "operands on different devices"
+    assert d == (torch.cuda.current_device() if _raw_device is None else _raw_device()), \
+        "operands on cuda:%d, which is not the current device" % d
 
 
 def _vector(t, n, dtype, name):
-    """An optional contiguous vector of n entries."""
-    assert t is None or (t.dtype == dtype and t.is_contiguous() and t.numel() == n), \
-        "%s must be %d contiguous %s" % (name, n, dtype)
-    return _ptr(t)
+    """Pointer of an optional contiguous vector of n entries."""
+    if t is None:
+        return None
+    assert t.dtype == dtype and t.numel() == n and t.is_contiguous(), "%s must be %d contiguous %s" % (name, n, dtype)
+    return t.data_ptr()
 
 
 def _f32c(t):
@@ -374,17 +373,23 @@ def gemm_f16x2(a_pieces, a_descale, b_pieces, b_descale, out, k, bias=None):
     return out
 
 
+def _fp8_bytes(rows, k):
+    """(icrl_fp8_piece_bytes, icrl_fp8_scale_bytes): 32 rows and 128 k at a time; a scale word holds four blocks of 128."""
+    rows = (rows + 31) // 32 * 32
+    blocks = (k + 127) // 128
+    return rows * blocks * 128, rows * ((blocks + 3) // 4) * 4
+
+
 def fp8_pieces(rows, k, device):
     """Buffers (pieces, scales) for a [rows, k] operand of gemm_fp8; cut_fp8 writes them whole."""
     assert rows > 0 and k > 0, "an 8-bit operand needs rows and columns"
-    return (torch.empty(load().icrl_fp8_piece_bytes(rows, k), dtype=torch.uint8, device=device),
-            torch.empty(load().icrl_fp8_scale_bytes(rows, k), dtype=torch.uint8, device=device))
+    return tuple(torch.empty(count, dtype=torch.uint8, device=device) for count in _fp8_bytes(rows, k))
 
 
 def _fp8_operand(pieces, scales, rows, k):
+    need = _fp8_bytes(rows, k)
     assert pieces.dtype == scales.dtype == torch.uint8 and pieces.is_contiguous() and scales.is_contiguous()
-    assert pieces.numel() >= load().icrl_fp8_piece_bytes(rows, k) > 0 and scales.numel() >= load().icrl_fp8_scale_bytes(rows, k), \
-        "8-bit buffers too small for [%d, %d]" % (rows, k)
+    assert pieces.numel() >= need[0] and scales.numel() >= need[1], "8-bit buffers too small for [%d, %d]" % (rows, k)
 
 
 def cut_fp8(x, pieces, scales):
@@ -393,20 +398,24 @@ def cut_fp8(x, pieces, scales):
     rows, k = x.shape
     _on_current_device(x, pieces, scales)
     _fp8_operand(pieces, scales, rows, k)
-    _check(load().icrl_cut_fp8(_ptr(x), _dtype_code(x), _row_stride(x), rows, k, _ptr(pieces), _ptr(scales), _stream()),
-           "icrl_cut_fp8")
+    _check(load().icrl_cut_fp8(x.data_ptr(), _dtype_code(x), _row_stride(x), rows, k, pieces.data_ptr(), scales.data_ptr(),
+                               _stream()), "icrl_cut_fp8")
 
 
 def gemm_fp8(a_pieces, a_scales, b_pieces, b_scales, out, k, bias=None):
     """out[M, N] = A . B^T (+ bias) from operands cut by cut_fp8 as [M, k] and [N, k]; out float32, bfloat16 or float16,
     float32 sums, one rounding at the end."""
     m, n = out.shape
-    _on_current_device(a_pieces, a_scales, b_pieces, b_scales, out, bias)
+    _on_current_device(out, a_pieces, a_scales, b_pieces, b_scales, bias)
     _fp8_operand(a_pieces, a_scales, m, k)
     _fp8_operand(b_pieces, b_scales, n, k)
-    with _Timed("gemm_fp8", 2.0 * m * n * k, m * k + k * n + float(out.element_size()) * m * n):
-        rc = load().icrl_gemm_fp8(_ptr(a_pieces), _ptr(a_scales), _ptr(b_pieces), _ptr(b_scales), _ptr(out), _dtype_code(out),
-                                  _row_stride(out), m, n, k, _vector(bias, n, torch.float32, "bias"), _stream())
+    args = (a_pieces.data_ptr(), a_scales.data_ptr(), b_pieces.data_ptr(), b_scales.data_ptr(), out.data_ptr(),
+            _dtype_code(out), _row_stride(out), m, n, k, _vector(bias, n, torch.float32, "bias"), _stream())
+    if PROFILE is None:
+        rc = load().icrl_gemm_fp8(*args)
+    else:
+        with _Timed("gemm_fp8", 2.0 * m * n * k, m * k + k * n + float(out.element_size()) * m * n):
+            rc = load().icrl_gemm_fp8(*args)
     _check(rc, "icrl_gemm_fp8")
     return out
 
@@ -575,30 +584,31 @@ def sample_tokens_filtered(logits, tokens_out, token_stride, uniforms, *, temper
     setting is a number or an [N] tensor (float32; top_k int32).  Temperature 0: the first largest entry.  token -1 and
     log_prob NaN: the row holds a NaN or nothing above -inf, or its settings are out of range."""
     n, v = logits.shape
-    _on_current_device(logits, tokens_out, uniforms, temperature, top_k, top_p, min_p, log_prob)
+    _on_current_device(logits, tokens_out, uniforms, log_prob)
     assert tokens_out.dtype == torch.int64 and _holds(tokens_out, n, token_stride), "tokens_out: int64, one place per row"
     assert log_prob is None or (log_prob.dtype == torch.float32 and _holds(log_prob, n, log_prob_stride)), \
         "log_prob: float32, one place per row"
     assert uniforms is not None
-
-    def setting(value, dtype, name):
-        if torch.is_tensor(value):
-            return _vector(value, n, dtype, name), 0
-        return None, value
-
-    t_rows, t = setting(temperature, torch.float32, "temperature")
-    k_rows, k = setting(top_k, torch.int32, "top_k")
-    p_rows, p = setting(top_p, torch.float32, "top_p")
-    m_rows, m = setting(min_p, torch.float32, "min_p")
-    _check(load().icrl_sample_tokens_filtered(_ptr(logits), _dtype_code(logits), _row_stride(logits), n, v,
-                                              _vector(uniforms, n, torch.float64, "uniforms"), t_rows, float(t), k_rows,
-                                              min(int(k), v), p_rows, float(p), m_rows, float(m), _ptr(tokens_out),
-                                              token_stride, _ptr(log_prob), log_prob_stride, _stream()),
+    rows, all_ = [None] * 4, [temperature, top_k, top_p, min_p]
+    for i, (dtype, name) in enumerate(_SETTINGS):
+        if isinstance(all_[i], torch.Tensor):
+            _on_current_device(logits, all_[i])
+            rows[i], all_[i] = _vector(all_[i], n, dtype, name), 0
+    _check(load().icrl_sample_tokens_filtered(logits.data_ptr(), _dtype_code(logits), _row_stride(logits), n, v,
+                                              _vector(uniforms, n, torch.float64, "uniforms"), rows[0], all_[0], rows[1],
+                                              min(int(all_[1]), v), rows[2], all_[2], rows[3], all_[3],
+                                              tokens_out.data_ptr(), token_stride,
+                                              None if log_prob is None else log_prob.data_ptr(), log_prob_stride, _stream()),
            "icrl_sample_tokens_filtered")
+
+
+_SETTINGS = ((torch.float32, "temperature"), (torch.int32, "top_k"), (torch.float32, "top_p"), (torch.float32, "min_p"))
 
 
 def _holds(t, n, stride):
     """Whether a buffer that starts at t's first element has n places `stride` elements apart."""
+    if stride == 1 and t.dim() == 1 and t.numel() >= n and t.is_contiguous():
+        return True
     return stride >= 1 and t.untyped_storage().nbytes() // t.element_size() - t.storage_offset() >= (n - 1) * stride + 1
 
 

@@ -86,6 +86,8 @@ def test_fp8_buffer_sizes():
     assert lib.icrl_fp8_scale_bytes(1, 1) == 32 * 4 and lib.icrl_fp8_scale_bytes(33, 513) == 64 * 8
     assert lib.icrl_fp8_piece_bytes(0, 5) == 0 and lib.icrl_fp8_scale_bytes(5, 0) == 0
     assert lib.icrl_fp8_piece_bytes(1 << 20, 1 << 14) == 1 << 34   # past 32 bits
+    for rows, k in ((1, 1), (31, 128), (32, 129), (33, 512), (10000, 513), (1 << 20, 1 << 14)):
+        assert hip._fp8_bytes(rows, k) == (lib.icrl_fp8_piece_bytes(rows, k), lib.icrl_fp8_scale_bytes(rows, k))
 
 
 def test_bindings_refuse_host_tensors_and_wrong_types():
