@@ -169,15 +169,20 @@ __global__ __launch_bounds__(WAVES * 64) void gemm_fp8_rows(Operand a, Operand b
     }
 }
 
-// ---- tiles of (64 WM) x (64 WN) per workgroup of 2 x 2 waves, operands staged through LDS a block of 128 at a time, the
-// next block's copy in flight (straight into LDS) while the current one is multiplied
+// ---- tiles of (64 WM) x (64 WN) per workgroup of 2 x 2 waves
+// Operands are staged through LDS 64 of k at a time in four buffers, copied there without passing registers: three stages
+// (of 1024 clocks of matrix instructions on 256 x 256 tiles) are in flight while one is multiplied, which covers the
+// latency of the caches behind the L2.  The fragments of the next stage are read from LDS into registers while the
+// current ones are multiplied, so one wave per SIMD keeps the matrix cores busy.
 template <typename T, int WM, int WN>
 __global__ __launch_bounds__(256) void gemm_fp8_tiles(Operand a, Operand b, T* __restrict__ out, int64_t ldo, int M, int N,
                                                       int nblocks, int words, const float* __restrict__ bias, int tiles_m,
                                                       int tiles_n) {
     constexpr int RA = 2 * WM, RB = 2 * WN;                 // 32-row blocks per tile
-    constexpr int STAGE = (RA + RB) * 4096;                 // bytes of one block of 128
-    __shared__ __attribute__((aligned(16))) unsigned char lds[2 * STAGE];
+    constexpr int STAGE = (RA + RB) * 2048, DEPTH = 4;      // bytes of one stage of 64; buffers
+    constexpr int COPIES = (RA + RB) / 2;                   // 16-byte copies per thread and stage
+    constexpr int BUFFERS = DEPTH * STAGE, SCALES = (RA + RB) * 128;   // scales: a word per row for 512 of k, in two buffers
+    __shared__ __attribute__((aligned(16))) unsigned char lds[BUFFERS + 2 * SCALES];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave >> 1, wn = wave & 1;
     // workgroups go round the 8 XCDs: give each XCD a contiguous run of tiles, in bands of 8 tile rows, so that what
     // its L2 holds is shared by the tiles it works on
@@ -189,72 +194,120 @@ __global__ __launch_bounds__(256) void gemm_fp8_tiles(Operand a, Operand b, T* _
     }
     const int band = t / (8 * tiles_n), in_band = t % (8 * tiles_n), rows_in_band = min(8, tiles_m - 8 * band);
     const int tm = 8 * band + in_band % rows_in_band, tn = in_band / rows_in_band;
-    auto stage = [&](int blk, int buf) {
-        unsigned char* base = lds + buf * STAGE;
+    // a stage is RA + RB pieces of 2 KB; wave w copies the (w & 1)-th KB of every second piece
+    const unsigned char* from[COPIES];
 #pragma unroll
-        for (int q = 0; q < RA + RB; ++q) {
-            // one 4 KB piece (a row block's block of 128) per step: each wave copies 1 KB of it
-            const bool is_a = q < RA;
-            const Operand& o = is_a ? a : b;
-            const int rb = min(is_a ? tm * RA + q : tn * RB + (q - RA), o.row_blocks - 1);   // past the end: any rows, never stored
-            const unsigned char* src = o.pieces + ((int64_t)rb * nblocks + blk) * 4096 + wave * 1024 + lane * 16;
-            unsigned char* dst = base + q * 4096 + wave * 1024;
-            __builtin_amdgcn_global_load_lds(reinterpret_cast<const __attribute__((address_space(1))) unsigned*>(reinterpret_cast<uintptr_t>(src)),
-                                             (__attribute__((address_space(3))) unsigned*)dst, 16, 0, 0);
-        }
+    for (int q = 0; q < COPIES; ++q) {
+        const int piece = 2 * q + (wave >> 1);
+        const bool is_a = piece < RA;
+        const Operand& o = is_a ? a : b;
+        const int rb = min(is_a ? tm * RA + piece : tn * RB + (piece - RA), o.row_blocks - 1);   // past the end: any rows, never stored
+        from[q] = o.pieces + (int64_t)rb * nblocks * 4096 + (wave & 1) * 1024 + lane * 16;
+    }
+    const int stages = 2 * nblocks;
+    auto stage = [&](int s) {
+        unsigned char* base = lds + (s % DEPTH) * STAGE + (wave >> 1) * 2048 + (wave & 1) * 1024;
+#pragma unroll
+        for (int q = 0; q < COPIES; ++q)
+            __builtin_amdgcn_global_load_lds(
+                reinterpret_cast<const __attribute__((address_space(1))) unsigned*>(reinterpret_cast<uintptr_t>(from[q] + (int64_t)s * 2048)),
+                (__attribute__((address_space(3))) unsigned*)(base + q * 4096), 16, 0, 0);
+    };
+    // scale words of one 512 of k: 128 bytes a row block, eight row blocks a wave
+    const unsigned char* scales_from;
+    {
+        const int piece = min(8 * wave + lane / 8, RA + RB - 1);
+        const bool is_a = piece < RA;
+        const Operand& o = is_a ? a : b;
+        const int rb = min(is_a ? tm * RA + piece : tn * RB + (piece - RA), o.row_blocks - 1);
+        scales_from = reinterpret_cast<const unsigned char*>(o.scales) + (int64_t)rb * words * 128 + (lane & 7) * 16;
+    }
+    auto stage_scales = [&](int word) {
+        if (wave < (RA + RB) / 8)
+            __builtin_amdgcn_global_load_lds(
+                reinterpret_cast<const __attribute__((address_space(1))) unsigned*>(reinterpret_cast<uintptr_t>(scales_from + (int64_t)word * 128)),
+                (__attribute__((address_space(3))) unsigned*)(lds + BUFFERS + (word & 1) * SCALES + wave * 1024), 16, 0, 0);
     };
     f32x16 acc[WM][WN] = {};
-    const unsigned* sa[WM];
-    const unsigned* sb[WN];
+    struct Raw { i32x4 a[WM][2], b[WN][2]; } raw[2];
+    auto fetch = [&](int s, Raw& r) {
+        const unsigned char* base = lds + (s % DEPTH) * STAGE + lane * 16;
 #pragma unroll
-    for (int i = 0; i < WM; ++i) sa[i] = a.scales + (int64_t)min(tm * RA + wm * WM + i, a.row_blocks - 1) * words * 32 + (lane & 31);
+        for (int i = 0; i < WM; ++i)
 #pragma unroll
-    for (int i = 0; i < WN; ++i) sb[i] = b.scales + (int64_t)min(tn * RB + wn * WN + i, b.row_blocks - 1) * words * 32 + (lane & 31);
+            for (int h = 0; h < 2; ++h) r.a[i][h] = *reinterpret_cast<const i32x4*>(base + (wm * WM + i) * 2048 + h * 1024);
+#pragma unroll
+        for (int i = 0; i < WN; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) r.b[i][h] = *reinterpret_cast<const i32x4*>(base + (RA + wn * WN + i) * 2048 + h * 1024);
+    };
     unsigned ea[WM], eb[WN];
-    stage(0, 0);
-    for (int blk = 0; blk < nblocks; ++blk) {
-        if ((blk & 3) == 0) {
+    // this wave's copies up to a stage have landed (all but the `later` newest stages' copies; scales among them only make
+    // it wait for more), its reads too, and then everyone's
+    auto landed = [&](int later) {
+        if (later >= 2) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"i"(2 * COPIES) : "memory");
+        else if (later == 1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"i"(COPIES) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        asm volatile("s_barrier" ::: "memory");
+    };
+    stage_scales(0);
+    for (int s = 0; s < 3 && s < stages; ++s) stage(s);
+    landed(min(2, stages - 1));
+    fetch(0, raw[0]);
+    auto step = [&](int s, const Raw& now, Raw& then) {
+        if ((s & 7) == 0) {
+            const unsigned* e = reinterpret_cast<const unsigned*>(lds + BUFFERS + (s >> 3 & 1) * SCALES) + (lane & 31);
 #pragma unroll
-            for (int i = 0; i < WM; ++i) ea[i] = sa[i][(blk >> 2) * 32];
+            for (int i = 0; i < WM; ++i) ea[i] = e[(wm * WM + i) * 32];
 #pragma unroll
-            for (int i = 0; i < WN; ++i) eb[i] = sb[i][(blk >> 2) * 32];
+            for (int i = 0; i < WN; ++i) eb[i] = e[(RA + wn * WN + i) * 32];
         }
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // each wave waits for its own part of this block's copy,
-        __syncthreads();                                   // then for the others'; the other buffer is free by now
-        if (blk + 1 < nblocks) stage(blk + 1, (blk + 1) & 1);
-        const unsigned char* base = lds + (blk & 1) * STAGE + lane * 16;
-#pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-            auto fragment = [&](int rb, unsigned scale) {
-                const unsigned char* p = base + rb * 4096 + kk * 2048;
-                return Fragment<T>(*reinterpret_cast<const i32x4*>(p), *reinterpret_cast<const i32x4*>(p + 1024), scale);
-            };
-            Fragment<T> fb[WN];
-#pragma unroll
-            for (int j = 0; j < WN; ++j) fb[j] = fragment(RA + wn * WN + j, eb[j]);
-#pragma unroll
-            for (int i = 0; i < WM; ++i) {
-                const Fragment<T> fa = fragment(wm * WM + i, ea[i]);
-#pragma unroll
-                for (int j = 0; j < WN; ++j) multiply(fa, fb[j], acc[i][j]);
-            }
+        if (s + 1 < stages) {
+            landed(min(1, stages - 2 - s));   // stages s + 2 .. are newer than s + 1
+            // the buffer of stage s + 3 held stage s - 1, and the next scales' buffer the words before these: every wave
+            // had read them before this barrier
+            if (s + 3 < stages) stage(s + 3);
+            if ((s & 7) == 1 && s + 7 < stages) stage_scales((s >> 3) + 1);
+            fetch(s + 1, then);
         }
+        Fragment<T> fb[WN];
 #pragma unroll
-        for (int i = 0; i < WM; ++i) ea[i] >>= 8;
+        for (int j = 0; j < WN; ++j) fb[j] = Fragment<T>(now.b[j][0], now.b[j][1], eb[j]);
 #pragma unroll
-        for (int i = 0; i < WN; ++i) eb[i] >>= 8;
+        for (int i = 0; i < WM; ++i) {
+            const Fragment<T> fa(now.a[i][0], now.a[i][1], ea[i]);
+#pragma unroll
+            for (int j = 0; j < WN; ++j) multiply(fa, fb[j], acc[i][j]);
+        }
+        if (s & 1) {   // the next block of 128: the next byte of the words
+#pragma unroll
+            for (int i = 0; i < WM; ++i) ea[i] >>= 8;
+#pragma unroll
+            for (int i = 0; i < WN; ++i) eb[i] >>= 8;
+        }
+    };
+    for (int s = 0; s < stages; s += 2) {   // stages come in pairs: k is padded to 128
+        step(s, raw[0], raw[1]);
+        step(s + 1, raw[1], raw[0]);
     }
+    // a lane holds 16 rows of one column of each 32 x 32 tile: a store writes two rows of 32 entries
 #pragma unroll
     for (int j = 0; j < WN; ++j) {
         const int n = (tn * RB + wn * WN + j) * 32 + (lane & 31);
-        const float add = bias && n < N ? bias[n] : 0.f;
+        if (n >= N) continue;
+        const float add = bias ? bias[n] : 0.f;
 #pragma unroll
         for (int i = 0; i < WM; ++i) {
-            const int m0 = (tm * RA + wm * WM + i) * 32 + 4 * (lane >> 5);
+            const int m0 = (tm * RA + wm * WM + i) * 32, mine = m0 + 4 * (lane >> 5);
+            T* p = out + (int64_t)mine * ldo + n;
+            if (m0 + 32 <= M) {
 #pragma unroll
-            for (int q = 0; q < 16; ++q) {
-                const int m = m0 + 8 * (q >> 2) + (q & 3);
-                if (m < M && n < N) store_out(out + (int64_t)m * ldo + n, acc[i][j][q] + add);
+                for (int q = 0; q < 16; ++q) store_out(p + (8 * (q >> 2) + (q & 3)) * ldo, acc[i][j][q] + add);
+            } else {
+                for (int q = 0; q < 16; ++q) {
+                    const int d = 8 * (q >> 2) + (q & 3);
+                    if (mine + d < M) store_out(p + d * ldo, acc[i][j][q] + add);
+                }
             }
         }
     }
