@@ -21,6 +21,11 @@ using namespace icrl;
 constexpr int MAX_K = 1024, MAX_V = 1 << 18;   // the bitmap of a row of 2^18 words is 32 KB of LDS
 constexpr double LOG2E = 1.4426950408889634074;
 
+// e^x in float64 to 7e-12 of itself (any x: infinite above 1e4, zero below -1e4, NaN for NaN)
+__device__ __forceinline__ double exp_of(double x) {
+    return x != x ? x : exp2_scaled(fmin(fmax(x, -1e4), 1e4) * LOG2E, 0);
+}
+
 template <typename T>
 __device__ __forceinline__ T from_float(float x) { return (T)x; }   // round to nearest even
 
@@ -52,7 +57,8 @@ __device__ __forceinline__ void write_row(const Row<T, NT, NV, false>& row, T* d
 #pragma unroll
         for (int j = 0; j < VEC; ++j) o.e[j] = from_float<T>(f(Elem<T>::value(p.e[j])));
         if (at + VEC <= row.V) {
-            *reinterpret_cast<typename Row<T, NT, NV, false>::Words*>(dst + at) = __builtin_bit_cast(typename Row<T, NT, NV, false>::Words, o);
+            __builtin_nontemporal_store(__builtin_bit_cast(typename Row<T, NT, NV, false>::Words, o),
+                                        reinterpret_cast<typename Row<T, NT, NV, false>::Words*>(dst + at));
         } else {
 #pragma unroll
             for (int j = 0; j < VEC; ++j)
@@ -70,7 +76,7 @@ __device__ __forceinline__ void fill_row(T* dst, int V, float x) {
 #pragma unroll
     for (int j = 0; j < VEC; ++j) o.e[j] = from_float<T>(x);
     for (int at = threadIdx.x * VEC; at < V; at += NT * VEC) {
-        if (at + VEC <= V) *reinterpret_cast<Words*>(dst + at) = __builtin_bit_cast(Words, o);
+        if (at + VEC <= V) __builtin_nontemporal_store(__builtin_bit_cast(Words, o), reinterpret_cast<Words*>(dst + at));
         else
             for (int j = at; j < V; ++j) dst[j] = o.e[0];
     }
@@ -84,12 +90,12 @@ __device__ __forceinline__ void put_stats(double* stats, int r, double a, double
 }
 
 template <typename T, int NT, int NV>
-__global__ __launch_bounds__(NT) void distill_kernel(const T* logits, int64_t ld, int V,
+__global__ __launch_bounds__(NT, 4) void distill_kernel(const T* logits, int64_t ld, int V,
                                                      const float* __restrict__ t_values, const int64_t* __restrict__ t_indices,
                                                      int k, const float* __restrict__ t_lse, double per_t,
                                                      const float* __restrict__ row_weight, float* __restrict__ row_loss,
                                                      double* __restrict__ stats, T* dlogits, int64_t ldd) {
-    extern __shared__ unsigned bits[];   // (V + 31) / 32 words, then k floats: the gradient at the listed words
+    extern __shared__ unsigned bits[];   // (V + 31) / 32 words: which words are listed
     __shared__ double sums[NT / 64 * 4];
     __shared__ float red[NT / 64][2];
     __shared__ int bad;
@@ -107,23 +113,71 @@ __global__ __launch_bounds__(NT) void distill_kernel(const T* logits, int64_t ld
         if (dst) fill_row<T, NT>(dst, V, 0.f);
         return;
     }
+    // this thread's entries of the list (their logits gathered while the row is on its way)
+    constexpr int MINE = MAX_K / NT;
+    int index[MINE];   // -1: none, or absent; -2: past the vocabulary
+    float value[MINE], logit[MINE];
+#pragma unroll
+    for (int q = 0; q < MINE; ++q) {
+        const int j = tid + q * NT;
+        const int64_t i = j < k ? ti[j] : -1;
+        index[q] = i < 0 ? -1 : i < V ? (int)i : -2;
+        value[q] = index[q] >= 0 ? tv[j] : -INFINITY;
+    }
     Row<T, NT, NV, false> row;
     row.open(src, V);
+#pragma unroll
+    for (int q = 0; q < MINE; ++q)
+        logit[q] = index[q] >= 0 ? Elem<T>::value(__builtin_bit_cast(typename Elem<T>::Raw, src[index[q]])) : 0.f;
     const int words = (V + 31) / 32;
-    float* at_listed = reinterpret_cast<float*>(bits + words);
     for (int w = tid; w < words; w += NT) bits[w] = 0;
     if (tid == 0) bad = 0;
     __syncthreads();
-    // the list: a negative index is an absent entry; one past the vocabulary, or the same one twice, is an error that
-    // makes the row's results NaN
-    float t_top = -INFINITY, best = -INFINITY;
-    for (int j = tid; j < k; j += NT) {
-        const int64_t i = ti[j];
-        if (i < 0) continue;
-        if (i >= V || (atomicOr(&bits[i >> 5], 1u << (i & 31)) >> (i & 31) & 1u)) bad = 1;
-        else t_top = fmaxf(t_top, tv[j]);
+    // a negative index is an absent entry; one past the vocabulary, or the same one twice, is an error that makes the
+    // row's results NaN
+    float t_top = -INFINITY;
+#pragma unroll
+    for (int q = 0; q < MINE; ++q) {
+        if (index[q] == -2) bad = 1;
+        if (index[q] >= 0) {
+            if (atomicOr(&bits[index[q] >> 5], 1u << (index[q] & 31)) >> (index[q] & 31) & 1u) bad = 1;
+            t_top = fmaxf(t_top, value[q]);
+        }
     }
-    row.each([&](float x, int) { best = fmaxf(best, x); });
+    // the sum outside the list.  A row in registers: its largest entry first.  A row that is read again by every pass: in
+    // one pass, every thread's sum relative to its own largest entry so far
+    constexpr bool ONLINE = NV == IN_MEMORY;
+    const float c = (float)(per_t * LOG2E);
+    float best = -INFINITY, part = 0.f;
+    auto outside_sum = [&](const auto& p, int at, float top) {   // a vector's entries share a word of the bitmap
+        const unsigned listed = at < V ? bits[at >> 5] >> (at & 31) : 0u;
+        float s = 0.f;
+#pragma unroll
+        for (int j = 0; j < Elem<T>::VEC; ++j) {
+            const float e = __builtin_amdgcn_exp2f((Elem<T>::value(p.e[j]) - top) * c);
+            s += listed >> j & 1u ? 0.f : e;
+        }
+        return s;
+    };
+    if constexpr (ONLINE) {
+        __syncthreads();   // the bitmap is whole
+        row.each_pack([&](const auto& p, int at) {
+            float top = best;
+#pragma unroll
+            for (int j = 0; j < Elem<T>::VEC; ++j) top = fmaxf(top, Elem<T>::value(p.e[j]));
+            if (top == -INFINITY) {   // nothing yet but -inf, or NaN, which fmaxf passes over
+#pragma unroll
+                for (int j = 0; j < Elem<T>::VEC; ++j)
+                    if (Elem<T>::value(p.e[j]) != Elem<T>::value(p.e[j])) part = NAN;
+                return;
+            }
+            part = part * (best == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((best - top) * c)) + outside_sum(p, at, top);
+            best = top;
+        });
+    } else {
+        row.each([&](float x, int) { best = fmaxf(best, x); });
+    }
+    float own = best;
     t_top = wave_max(t_top);
     best = wave_max(best);
     if (lane == 0) { red[wave][0] = t_top; red[wave][1] = best; }
@@ -138,29 +192,23 @@ __global__ __launch_bounds__(NT) void distill_kernel(const T* logits, int64_t ld
         if (dst) fill_row<T, NT>(dst, V, NAN);
         return;
     }
-    // sums outside the list and over it
-    const float c = (float)(per_t * LOG2E);
-    float part = 0.f;
-    row.each_pack([&](const auto& p, int at) {   // a vector's entries share a word of the bitmap
-        const unsigned listed = at < V ? bits[at >> 5] >> (at & 31) : 0u;
-#pragma unroll
-        for (int j = 0; j < Elem<T>::VEC; ++j) {
-            const float e = __builtin_amdgcn_exp2f((Elem<T>::value(p.e[j]) - best) * c);
-            part += listed >> j & 1u ? 0.f : e;
-        }
-    });
+    if constexpr (ONLINE) {
+        if (own > -INFINITY) part *= __builtin_amdgcn_exp2f((own - best) * c);
+    } else {
+        row.each_pack([&](const auto& p, int at) { part += outside_sum(p, at, best); });
+    }
+    // sums over the list: its part of Z, u_j = e^(t_j / T - t_ref), u_j (log u_j - z_j)
     const bool tail = t_lse != nullptr;
-    const double t_ref = tail ? (double)t_lse[r] : (double)t_top * per_t;   // u_j = e^(t_j / T - t_ref)
-    double s[4] = {(double)part, 0.0, 0.0, 0.0};   // outside; listed; sum u; sum u (log u - (x - best) / T)
-    for (int j = tid; j < k; j += NT) {
-        const int64_t i = ti[j];
-        if (i < 0) continue;
-        const float x = Elem<T>::value(__builtin_bit_cast(typename Elem<T>::Raw, src[i]));
-        const double z = ((double)x - (double)best) * per_t, d = (double)tv[j] * per_t - t_ref;
-        const double u = exp(d);
-        s[1] += exp(z);
-        s[2] += u;
-        if (u != 0.0) s[3] += u * (d - z);
+    const double t_ref = tail ? (double)t_lse[r] : (double)t_top * per_t;
+    double s[4] = {(double)part, 0.0, 0.0, 0.0}, e_listed[MINE], u_listed[MINE];
+#pragma unroll
+    for (int q = 0; q < MINE; ++q) {
+        const double z = ((double)logit[q] - (double)best) * per_t, d = (double)value[q] * per_t - t_ref;
+        e_listed[q] = index[q] >= 0 ? exp_of(z) : 0.0;
+        u_listed[q] = index[q] >= 0 ? exp_of(d) : 0.0;
+        s[1] += e_listed[q];
+        s[2] += u_listed[q];
+        if (u_listed[q] != 0.0) s[3] += u_listed[q] * (d - z);
     }
     block_sums<NT, 4>(s, sums);
     const double Z = s[0] + s[1], log_z = log(Z), U = s[2];
@@ -191,22 +239,19 @@ __global__ __launch_bounds__(NT) void distill_kernel(const T* logits, int64_t ld
         if (stats) put_stats(stats, r, (double)best * per_t + log_z, teacher, W, W - ratio);
     }
     if (!dst) return;
-    const double g = (double)weight * per_t;
-    for (int j = tid; j < k; j += NT) {   // before the first write: dlogits may be the logits themselves
-        const int64_t i = ti[j];
-        if (i < 0) continue;
-        const float x = Elem<T>::value(__builtin_bit_cast(typename Elem<T>::Raw, src[i]));
-        const double p = exp(((double)x - (double)best) * per_t) / Z, q = q_scale != 0.0 ? exp((double)tv[j] * per_t - t_ref) * q_scale : 0.0;
-        at_listed[j] = (float)(g * (p * W - q));
+    if (W == 0.0) {
+        fill_row<T, NT>(dst, V, 0.f);
+        return;
     }
-    __syncthreads();
+    const double g = (double)weight * per_t;
+    __syncthreads();   // dlogits may be the logits themselves: every gathered logit is in its thread's hands
     const float outside = (float)(g * (W - ratio) / Z);
     write_row<T, NT, NV>(row, dst, [&](float x) { return outside * __builtin_amdgcn_exp2f((x - best) * c); });
     __syncthreads();   // the row's writes come before those at the listed words
-    for (int j = tid; j < k; j += NT) {
-        const int64_t i = ti[j];
-        if (i >= 0) dst[i] = from_float<T>(at_listed[j]);
-    }
+#pragma unroll
+    for (int q = 0; q < MINE; ++q)
+        if (index[q] >= 0)
+            dst[index[q]] = from_float<T>((float)(g * (e_listed[q] / Z * W - u_listed[q] * q_scale)));
 }
 
 // The gradient alone, from the forward pass's stats.
@@ -223,12 +268,12 @@ __global__ __launch_bounds__(NT) void distill_grad_kernel(const T* logits, int64
     const int64_t* ti = t_indices + (int64_t)r * k;
     T* dst = dlogits + (int64_t)r * ldd;
     const float weight = row_weight ? row_weight[r] : 1.f;
-    if (weight == 0.f) {
+    const double log_z = stats[4 * (int64_t)r], teacher = stats[4 * (int64_t)r + 1], W = stats[4 * (int64_t)r + 2],
+                 W_out = stats[4 * (int64_t)r + 3];
+    if (weight == 0.f || W == 0.0) {   // W = 0: nothing to learn from this row, or idle in the forward pass
         fill_row<T, NT>(dst, V, 0.f);
         return;
     }
-    const double log_z = stats[4 * (int64_t)r], teacher = stats[4 * (int64_t)r + 1], W = stats[4 * (int64_t)r + 2],
-                 W_out = stats[4 * (int64_t)r + 3];
     Row<T, NT, NV, false> row;
     row.open(src, V);
     const double g = (double)weight * per_t;
@@ -236,7 +281,7 @@ __global__ __launch_bounds__(NT) void distill_grad_kernel(const T* logits, int64
         const int64_t i = ti[j];
         if (i < 0 || i >= V) continue;   // past the vocabulary: the stats are NaN already
         const float x = Elem<T>::value(__builtin_bit_cast(typename Elem<T>::Raw, src[i]));
-        const double p = exp((double)x * per_t - log_z), q = W != 0.0 ? exp((double)tv[j] * per_t - teacher) : 0.0;
+        const double p = exp_of((double)x * per_t - log_z), q = exp_of((double)tv[j] * per_t - teacher);
         at_listed[j] = (float)(g * (p * W - q));
     }
     __syncthreads();
@@ -278,7 +323,7 @@ extern "C" int icrl_distill_loss(const void* logits, int dtype, int64_t ld_logit
     ICRL_REQUIRE(row_loss, "icrl_distill_loss: null pointer or empty shape");
     ICRL_REQUIRE(reinterpret_cast<uintptr_t>(stats) % 8 == 0, "icrl_distill_loss: stats must be 8-byte aligned");
     ICRL_REQUIRE(!dlogits || ld_dlogits >= V, "icrl_distill_loss: ld_dlogits < V");
-    const size_t lds = ((size_t)(V + 31) / 32 + k) * 4;
+    const size_t lds = (size_t)((V + 31) / 32) * 4;
 #define ICRL_CALL(T, NT, NV)                                                                                            \
     hipLaunchKernelGGL((distill_kernel<T, NT, NV>), dim3(N), dim3(NT), lds, icrl::as_stream(stream),                    \
                        static_cast<const T*>(logits), ld_logits, V, teacher_values, teacher_indices, k, teacher_lse,    \

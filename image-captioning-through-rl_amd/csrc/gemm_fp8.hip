@@ -32,10 +32,10 @@ inline int scale_words(int K) { return (blocks128(K) + 3) / 4; }   // 32-bit wor
 
 // Eight lanes cut one row's block of 128: 16 entries a lane, which are one 16-byte half of the fragment's lane.
 template <typename T>
-__global__ __launch_bounds__(256) void cut_kernel(const T* __restrict__ x, int64_t ld, int rows, int K, int nblocks, int words,
+__global__ __launch_bounds__(64) void cut_kernel(const T* __restrict__ x, int64_t ld, int rows, int K, int nblocks, int words,
                                                   unsigned char* __restrict__ pieces, unsigned char* __restrict__ scales) {
     const int lane8 = threadIdx.x & 7;
-    const int64_t unit = (int64_t)blockIdx.x * 32 + (threadIdx.x >> 3);   // (row, group of four blocks' block)
+    const int64_t unit = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 3);   // (row, group of four blocks' block)
     const int padded = words * 4;
     const int row = (int)(unit / padded), b = (int)(unit % padded);
     if (row >= (rows + 31) / 32 * 32) return;
@@ -181,7 +181,9 @@ __global__ __launch_bounds__(256) void gemm_fp8_tiles(Operand a, Operand b, T* _
     constexpr int RA = 2 * WM, RB = 2 * WN;                 // 32-row blocks per tile
     constexpr int STAGE = (RA + RB) * 2048, DEPTH = 4;      // bytes of one stage of 64; buffers
     constexpr int COPIES = (RA + RB) / 2;                   // 16-byte copies per thread and stage
-    constexpr int BUFFERS = DEPTH * STAGE, SCALES = (RA + RB) * 128;   // scales: a word per row for 512 of k, in two buffers
+    constexpr bool WIDE = sizeof(T) == 2;                   // the products' tiles are transposed (see the end)
+    constexpr int SCALE_WAVES = (RA + RB + 7) / 8;           // waves that copy scales
+    constexpr int BUFFERS = DEPTH * STAGE, SCALES = SCALE_WAVES * 1024;   // scales: a word per row for 512 of k, in two buffers
     __shared__ __attribute__((aligned(16))) unsigned char lds[BUFFERS + 2 * SCALES];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave >> 1, wn = wave & 1;
     // workgroups go round the 8 XCDs: give each XCD a contiguous run of tiles, in bands of 8 tile rows, so that what
@@ -223,7 +225,7 @@ __global__ __launch_bounds__(256) void gemm_fp8_tiles(Operand a, Operand b, T* _
         scales_from = reinterpret_cast<const unsigned char*>(o.scales) + (int64_t)rb * words * 128 + (lane & 7) * 16;
     }
     auto stage_scales = [&](int word) {
-        if (wave < (RA + RB) / 8)
+        if (wave < SCALE_WAVES)
             __builtin_amdgcn_global_load_lds(
                 reinterpret_cast<const __attribute__((address_space(1))) unsigned*>(reinterpret_cast<uintptr_t>(scales_from + (int64_t)word * 128)),
                 (__attribute__((address_space(3))) unsigned*)(lds + BUFFERS + (word & 1) * SCALES + wave * 1024), 16, 0, 0);
@@ -251,8 +253,8 @@ __global__ __launch_bounds__(256) void gemm_fp8_tiles(Operand a, Operand b, T* _
         asm volatile("s_barrier" ::: "memory");
     };
     stage_scales(0);
-    for (int s = 0; s < 3 && s < stages; ++s) stage(s);
-    landed(min(2, stages - 1));
+    for (int s = 0; s < DEPTH - 1 && s < stages; ++s) stage(s);
+    landed(min(DEPTH - 2, stages - 1));
     fetch(0, raw[0]);
     auto step = [&](int s, const Raw& now, Raw& then) {
         if ((s & 7) == 0) {
@@ -263,10 +265,10 @@ __global__ __launch_bounds__(256) void gemm_fp8_tiles(Operand a, Operand b, T* _
             for (int i = 0; i < WN; ++i) eb[i] = e[(RA + wn * WN + i) * 32];
         }
         if (s + 1 < stages) {
-            landed(min(1, stages - 2 - s));   // stages s + 2 .. are newer than s + 1
-            // the buffer of stage s + 3 held stage s - 1, and the next scales' buffer the words before these: every wave
+            landed(min(DEPTH - 3, stages - 2 - s));   // stages s + 2 .. are newer than s + 1
+            // the buffer of stage s + DEPTH - 1 held stage s - 1, and the next scales' buffer the words before these: every wave
             // had read them before this barrier
-            if (s + 3 < stages) stage(s + 3);
+            if (s + DEPTH - 1 < stages) stage(s + DEPTH - 1);
             if ((s & 7) == 1 && s + 7 < stages) stage_scales((s >> 3) + 1);
             fetch(s + 1, then);
         }
@@ -277,7 +279,10 @@ __global__ __launch_bounds__(256) void gemm_fp8_tiles(Operand a, Operand b, T* _
         for (int i = 0; i < WM; ++i) {
             const Fragment<T> fa(now.a[i][0], now.a[i][1], ea[i]);
 #pragma unroll
-            for (int j = 0; j < WN; ++j) multiply(fa, fb[j], acc[i][j]);
+            for (int j = 0; j < WN; ++j) {
+                if (WIDE) multiply(fb[j], fa, acc[i][j]);
+                else multiply(fa, fb[j], acc[i][j]);
+            }
         }
         if (s & 1) {   // the next block of 128: the next byte of the words
 #pragma unroll
@@ -290,7 +295,62 @@ __global__ __launch_bounds__(256) void gemm_fp8_tiles(Operand a, Operand b, T* _
         step(s, raw[0], raw[1]);
         step(s + 1, raw[1], raw[0]);
     }
-    // a lane holds 16 rows of one column of each 32 x 32 tile: a store writes two rows of 32 entries
+    if constexpr (WIDE) {
+        // 16-bit outputs: a lane holds four neighbouring columns of a row at a time (the transposed product's rows), which
+        // go through LDS, so that a store writes 16 bytes a lane and whole lines of a row; one by one they would be written
+        // in 64-byte pieces (4096 x 32000 x 2048: 356 us so, 330 through LDS).  Rows are 8 bytes apart from a multiple of
+        // the banks.
+        constexpr int COLS = 32 * WN, PITCH = COLS * 2 + 8;
+        static_assert(4 * 32 * WM * PITCH <= (int)sizeof(lds), "the waves' tiles fit the stages' place");
+        unsigned char* mine = lds + wave * (32 * WM * PITCH);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __syncthreads();   // every wave has read its last stage
+#pragma unroll
+        for (int j = 0; j < WN; ++j) {
+            float add[4][4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int n = (tn * RB + wn * WN + j) * 32 + 8 * q + 4 * (lane >> 5) + e;
+                    add[q][e] = bias && n < N ? bias[n] : 0.f;
+                }
+#pragma unroll
+            for (int i = 0; i < WM; ++i)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    struct alignas(8) Four { T e[4]; } four;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) four.e[e] = (T)(acc[i][j][4 * q + e] + add[q][e]);
+                    *reinterpret_cast<Four*>(mine + (32 * i + (lane & 31)) * PITCH + (32 * j + 8 * q + 4 * (lane >> 5)) * 2) = four;
+                }
+        }
+        // (a wave reads back its own tile only: no barrier)
+        constexpr int PER_ROW = COLS / 8, ROWS = 64 / PER_ROW;   // lanes per row, rows per store
+        const int m0 = (tm * RA + wm * WM) * 32, n0 = (tn * RB + wn * WN) * 32 + lane % PER_ROW * 8;
+        typedef unsigned Words __attribute__((ext_vector_type(4), aligned(2), may_alias));
+        typedef unsigned Pair __attribute__((ext_vector_type(2), may_alias));
+#pragma unroll 4
+        for (int row = lane / PER_ROW; row < 32 * WM; row += ROWS) {
+            const Pair* from = reinterpret_cast<const Pair*>(mine + row * PITCH + lane % PER_ROW * 16);
+            const Pair lo = from[0], hi = from[1];
+            Words w = {lo[0], lo[1], hi[0], hi[1]};
+            T* to = out + (int64_t)(m0 + row) * ldo + n0;
+            if (m0 + row < M) {
+                if (n0 + 8 <= N) {
+                    *reinterpret_cast<Words*>(to) = w;
+                } else {
+                    struct Eight { T e[8]; };
+                    const Eight v = __builtin_bit_cast(Eight, w);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (n0 + e < N) to[e] = v.e[e];
+                }
+            }
+        }
+        return;
+    }
+    // float32 outputs: a lane holds 16 rows of one column of each 32 x 32 tile: a store writes two whole lines
 #pragma unroll
     for (int j = 0; j < WN; ++j) {
         const int n = (tn * RB + wn * WN + j) * 32 + (lane & 31);
@@ -304,6 +364,7 @@ __global__ __launch_bounds__(256) void gemm_fp8_tiles(Operand a, Operand b, T* _
 #pragma unroll
                 for (int q = 0; q < 16; ++q) store_out(p + (8 * (q >> 2) + (q & 3)) * ldo, acc[i][j][q] + add);
             } else {
+#pragma unroll
                 for (int q = 0; q < 16; ++q) {
                     const int d = 8 * (q >> 2) + (q & 3);
                     if (mine + d < M) store_out(p + d * ldo, acc[i][j][q] + add);
@@ -327,10 +388,10 @@ extern "C" int icrl_cut_fp8(const void* x, int dtype, int64_t ld, int rows, int 
     ICRL_REQUIRE(reinterpret_cast<uintptr_t>(pieces) % 16 == 0 && reinterpret_cast<uintptr_t>(scales) % 4 == 0,
                  "icrl_cut_fp8: pieces must be 16-byte aligned, scales 4-byte");
     const int words = scale_words(K), nb = blocks128(K);
-    const int64_t units = (int64_t)((rows + 31) / 32 * 32) * words * 4, grid = (units + 31) / 32;
+    const int64_t units = (int64_t)((rows + 31) / 32 * 32) * words * 4, grid = units / 8;
     ICRL_REQUIRE(grid <= 0x7FFFFFFF, "icrl_cut_fp8: operand too large");
 #define ICRL_CALL(T)                                                                                              \
-    hipLaunchKernelGGL((cut_kernel<T>), dim3((unsigned)grid), dim3(256), 0, icrl::as_stream(stream),              \
+    hipLaunchKernelGGL((cut_kernel<T>), dim3((unsigned)grid), dim3(64), 0, icrl::as_stream(stream),               \
                        static_cast<const T*>(x), ld, rows, K, nb, words, static_cast<unsigned char*>(pieces),     \
                        static_cast<unsigned char*>(scales))
     switch (dtype) {
@@ -353,15 +414,21 @@ void launch_gemm(const Operand& a, const Operand& b, T* out, int64_t ldo, int M,
                            words, bias);
         return;
     }
-    const int big_m = (M + 255) / 256, big_n = (N + 255) / 256;
-    if ((int64_t)big_m * big_n >= 512) {
-        hipLaunchKernelGGL((gemm_fp8_tiles<T, 4, 4>), dim3(big_m * big_n), dim3(256), 0, st, a, b, out, ldo, M, N, nb, words,
-                           bias, big_m, big_n);
-    } else {
-        const int tm = (M + 127) / 128, tn = (N + 127) / 128;
-        hipLaunchKernelGGL((gemm_fp8_tiles<T, 2, 2>), dim3(tm * tn), dim3(256), 0, st, a, b, out, ldo, M, N, nb, words, bias,
-                           tm, tn);
-    }
+#define ICRL_TILES(WM, WN)                                                                                                     \
+    do {                                                                                                                       \
+        const int tm = (M + 64 * WM - 1) / (64 * WM), tn = (N + 64 * WN - 1) / (64 * WN);                                      \
+        hipLaunchKernelGGL((gemm_fp8_tiles<T, WM, WN>), dim3(tm * tn), dim3(256), 0, st, a, b, out, ldo, M, N, nb, words, bias, \
+                           tm, tn);                                                                                            \
+    } while (0)
+    // Measured (us; 256 x 256, 128 x 128 and 64 x 128 tiles): 4096 x 32000 x 2048 330 / 340 / 380, the same at k = 128
+    // 98 / 86 / 89, 2048 x 10000 x 2048 80 / 57 / 65, 512 x 10000 x 512 (float32 out) 23 / 13.5 / 12, 1024 x 4096 x 4096
+    // 69 / 32 / 30.  The largest tiles have one workgroup per CU and need many rounds of a long k to make up for their
+    // ends; the smallest ones spread better when there are fewer than three of the middle ones per CU.
+    const int64_t tiles256 = (int64_t)((M + 255) / 256) * ((N + 255) / 256), tiles128 = (int64_t)((M + 127) / 128) * ((N + 127) / 128);
+    if (tiles256 >= 1024 && K >= 2048) ICRL_TILES(4, 4);
+    else if (tiles128 >= 768) ICRL_TILES(2, 2);
+    else ICRL_TILES(1, 2);
+#undef ICRL_TILES
 }
 }  // namespace
 

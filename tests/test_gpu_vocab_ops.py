@@ -344,6 +344,29 @@ def test_distillation_bad_lists_and_rows_are_nan():
     assert torch.isnan(later[:5]).all() and torch.isfinite(later[5]).all()
 
 
+@pytest.mark.parametrize("v", [700, 70000])   # in registers, and read again
+def test_distillation_nan_rows_and_rows_with_nothing_to_learn(v):
+    k = 5
+    x = rows_of(4, v, F32, 13)
+    x[0, :] = -INF
+    x[0, 40] = NAN                 # among nothing else
+    x[1, v - 1] = NAN
+    x[2] = -INF
+    tv, ti, lse = teacher_for(x.nan_to_num(0.0), k, 1.0, 14)
+    ti[0] = torch.arange(k).cuda() + 50
+    ti[2] = -1                     # no entry, and a row without mass
+    for given in (lse, None):
+        loss, grad = torch.empty(4, device="cuda"), torch.empty_like(x)
+        stats = torch.empty(4, 4, dtype=torch.float64, device="cuda")
+        hip.distill_loss(x, tv, ti, loss, teacher_lse=given, dlogits=grad, stats=stats)
+        later = torch.empty_like(x)
+        hip.distill_grad(x, tv, ti, stats, later)
+        assert torch.isnan(loss[:2]).all() and torch.isnan(grad[:2]).all() and torch.isnan(later[:2]).all()
+        if given is None:
+            assert loss[2].item() == 0.0 and (grad[2] == 0).all() and (later[2] == 0).all()
+        check_distill(x[3:], tv[3:], ti[3:], None if given is None else given[3:], 1.0, None, loss[3:], grad[3:])
+
+
 def test_distillation_masked_words_and_sure_rows():
     v, k = 4000, 8
     x = rows_of(4, v, F32, 8)
