@@ -37,7 +37,6 @@ struct Shared {
     u64 above, cut, total;
     float red[NT / 64];
     int flag;
-    float bound;
 };
 
 __device__ __forceinline__ u64 composite(unsigned key, int index) { return (u64)key << 32 | (unsigned)~index; }
@@ -228,6 +227,7 @@ __device__ __forceinline__ u64 ranked(int n, Shared<NT>& sm) {
             const u64 mine = sm.hist[tid];
             const ulonglong2* two = reinterpret_cast<const ulonglong2*>(sm.hist);
             int rank = 0;
+#pragma unroll 8
             for (int j = 0; j < (n + 1) / 2; ++j) {
                 const ulonglong2 o = two[j];
                 rank += (o.x > mine) + (o.y > mine);
@@ -369,52 +369,81 @@ __device__ __forceinline__ u64 find_cut(const R& row, Shared<NT>& sm, bool by_ma
 }
 
 // A value that at least k entries of the row reach (k <= NT), not far below the k-th largest: the k-th largest of the
-// threads' own maxima, cut to its key's upper 16 bits.  One wave finds it, a bit at a time.  -inf: fewer than k threads
-// hold an entry above it.
+// threads' own maxima, cut to its key's upper 16 bits.  Four bits a step: the waves share out the 16 continuations of
+// what is known (0.5 us; a single wave, bit by bit, takes 1.9).  -inf: fewer than k threads hold an entry above it.
 template <int NT>
 __device__ __forceinline__ float bound_of(float own_max, int k, Shared<NT>& sm) {
+    constexpr int WAVES = NT / 64, PER = 16 / WAVES;   // continuations a wave counts
     unsigned* keys = reinterpret_cast<unsigned*>(sm.hist);
+    int* reached = reinterpret_cast<int*>(sm.hist + BINS / 2);   // 16 counts a step
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     __syncthreads();
-    keys[threadIdx.x] = order_key(own_max);
+    keys[threadIdx.x] = order_key(own_max) >> 16;
     __syncthreads();
-    if (threadIdx.x < 64) {
-        unsigned key[NT / 64], t = 0;
+    unsigned key[WAVES], t = 0;
 #pragma unroll
-        for (int i = 0; i < NT / 64; ++i) key[i] = keys[threadIdx.x + 64 * i] >> 16;
-        for (unsigned bit = 0x8000u; bit; bit >>= 1) {
-            int reached = 0;
+    for (int i = 0; i < WAVES; ++i) key[i] = keys[lane + 64 * i];
 #pragma unroll
-            for (int i = 0; i < NT / 64; ++i) reached += __popcll(__ballot(key[i] >= (t | bit)));
-            if (reached >= k) t |= bit;
+    for (int step = 0; step < 4; ++step) {
+        const int shift = 12 - 4 * step;
+#pragma unroll
+        for (int c = 0; c < PER; ++c) {
+            const unsigned at_least = t | (unsigned)(wave * PER + c) << shift;
+            int n = 0;
+#pragma unroll
+            for (int i = 0; i < WAVES; ++i) n += __popcll(__ballot(key[i] >= at_least));
+            if (lane == 0) reached[16 * step + wave * PER + c] = n;
         }
-        if (threadIdx.x == 0) {
-            t <<= 16;
-            // between two upper halves lies -inf's: what rounds down to it or below says nothing
-            sm.bound = t <= kKeyMinusInf ? -INFINITY : value_of((u64)t << 32);
-        }
+        __syncthreads();
+        // counts fall as the continuation rises: the last that k maxima reach
+        const int n = lane < 16 ? reached[16 * step + lane] : 0;
+        const int last = __popcll(__ballot(lane < 16 && n >= k)) - 1;
+        t |= (unsigned)max(last, 0) << shift;   // (none: fewer than k maxima, which only step 0 can say; t stays 0)
     }
-    __syncthreads();
-    return sm.bound;
+    t <<= 16;
+    // between two upper halves lies -inf's: what rounds down to it or below says nothing
+    return t <= kKeyMinusInf ? -INFINITY : value_of((u64)t << 32);
 }
 
-// Composites of the entries >= bound (> -inf) into sm.hist, at most `room` of them; returns how many there are.
+// Composites of the entries >= bound (> -inf) into sm.hist, at most `room` of them; returns how many there are.  A thread
+// keeps its first two to itself, so that nothing waits for the shared counter while it reads; only what a thread finds
+// beyond them goes through it one by one.
 template <int NT, typename R>
 __device__ __forceinline__ int collect(const R& row, Shared<NT>& sm, float bound, int room) {
+    const int lane = threadIdx.x & 63;
     __syncthreads();
     if (threadIdx.x == 0) sm.count = 0;
     __syncthreads();
+    u64 mine[2] = {0, 0};
+    int n = 0;
     row.each_pack([&](const typename R::Pack& p, int at) {
         float most = -INFINITY;
 #pragma unroll
         for (int j = 0; j < R::VEC; ++j) most = fmaxf(most, Elem<typename R::Type>::value(p.e[j]));
         if (!(most >= bound)) return;
-        row.vector(p, at, [&](float x, int i) {
+#pragma unroll
+        for (int j = 0; j < R::VEC; ++j) {
+            const float x = Elem<typename R::Type>::value(p.e[j]);
             if (x >= bound) {
-                const int to = atomicAdd(&sm.count, 1);
-                if (to < room) sm.hist[to] = composite(order_key(x), i);
+                const u64 c = composite(order_key(x), at + j);
+                if (n >= 2) {
+                    const int to = atomicAdd(&sm.count, 1);
+                    if (to < room) sm.hist[to] = c;
+                }
+                mine[1] = n == 1 ? c : mine[1];
+                mine[0] = n == 0 ? c : mine[0];
+                ++n;
             }
-        });
+        }
     });
+    n = min(n, 2);
+    const u64 one = __ballot(n >= 1), two = __ballot(n == 2), below = (1ull << lane) - 1;
+    int base = 0;
+    if (lane == 0) base = atomicAdd(&sm.count, __popcll(one) + __popcll(two));
+    base = __shfl(base, 0, 64) + __popcll(one & below) + __popcll(two & below);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        if (i < n && base + i < room) sm.hist[base + i] = mine[i];
     __syncthreads();
     return sm.count;
 }
@@ -543,6 +572,7 @@ __global__ __launch_bounds__(NT, 4) void sample_filtered_kernel(const T* __restr
             if (w) {
                 const unsigned mine = (unsigned)index_of(c);
                 u64 upto = 0;
+#pragma unroll 4
                 for (int j = 0; j < m; ++j) {
                     const Kept o = kept[j];
                     upto += o.index <= mine ? o.w : 0;
@@ -560,7 +590,7 @@ __global__ __launch_bounds__(NT, 4) void sample_filtered_kernel(const T* __restr
         const u64 w = weight(x);
         const bool in = (x > cut_x) | ((x == cut_x) & ((unsigned)i <= cut_index));
         const bool low = (x != best) & ((double)x - (double)best < floor_z);
-        return in & !low ? w : 0;
+        return (in & !low) ? w : 0;
     };
 
     // ---- the whole row
