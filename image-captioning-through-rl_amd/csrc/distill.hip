@@ -23,7 +23,8 @@ constexpr double LOG2E = 1.4426950408889634074;
 
 // e^x in float64 to 7e-12 of itself (any x: infinite above 1e4, zero below -1e4, NaN for NaN)
 __device__ __forceinline__ double exp_of(double x) {
-    return x != x ? x : exp2_scaled(fmin(fmax(x, -1e4), 1e4) * LOG2E, 0);
+    const double t = fmin(fmax(x, -1e4), 1e4) * LOG2E, n = rint(t);
+    return x != x ? x : ldexp(exp2_fraction(t - n), (int)n);
 }
 
 template <typename T>

@@ -53,7 +53,7 @@ struct Weights {
     int S;
     __device__ __forceinline__ double units(float x) const {   // before rounding
         const double t = ((double)fminf(x, 3.402823466e38f) - top) * per_unit;
-        return exp2_scaled(fmax(t, -(double)(S + 2)), S);       // at least 1/4, which rounds to nothing; at most 2^51
+        return exp2_normal(fmax(t, -(double)(S + 2)), S);       // at least 1/4, which rounds to nothing; at most 2^51
     }
     static __device__ __forceinline__ u64 rounded(double units) {   // the sum's low 52 bits: units to the nearest integer
         return (u64)__double_as_longlong(units + 0x1p52) & ((1ull << 52) - 1);
@@ -252,8 +252,13 @@ template <int NT, typename R, typename G>
 __device__ __forceinline__ u64 find_cut(const R& row, Shared<NT>& sm, bool by_mass, u64 from, const Weights& weight, float width,
                                         G&& need_of, u64& mass_kept) {
     constexpr int VEC = R::VEC;
-    const unsigned from_key = (unsigned)(from >> 32), from_index = ~(unsigned)from;
-    auto kept = [&](unsigned key, int i) { return key > from_key || (key == from_key && (unsigned)i <= from_index); };
+    // with values, not keys (a few instructions an entry less); NaN, which no comparison keeps, belongs to a whole row
+    const float from_x = value_of(from);
+    const unsigned from_index = ~(unsigned)from;
+    const bool whole = from_x != from_x;
+    auto kept = [&](float x, int i) {
+        return whole ? i < row.V : (x > from_x) | ((x == from_x) & ((unsigned)i <= from_index));
+    };
     auto amount = [&](float x) { return by_mass ? weight(x) : (u64)1; };
     const float per = (float)BINS / width, top = (float)weight.top;
     auto bin = [&](float x) {   // monotone in the row's order; what is far below the top, NaN included, is the last bin
@@ -280,7 +285,7 @@ __device__ __forceinline__ u64 find_cut(const R& row, Shared<NT>& sm, bool by_ma
         for (int j = 0; j < VEC; ++j) {
             const float x = Elem<typename R::Type>::value(p.e[j]);
             const int b = bin(x);
-            const bool in = kept(order_key(x), at + j);
+            const bool in = kept(x, at + j);
             rest += in && b == BINS - 1 ? a[j] : 0;
             if (in && b < BINS - 1) atomicAdd(&sm.hist[b], a[j]);
         }
@@ -302,7 +307,7 @@ __device__ __forceinline__ u64 find_cut(const R& row, Shared<NT>& sm, bool by_ma
         for (int j = 0; j < VEC; ++j) {
             const float x = Elem<typename R::Type>::value(p.e[j]);
             const int b = bin(x);
-            const bool in = kept(order_key(x), at + j);
+            const bool in = kept(x, at + j);
             sure += in && b < b0 ? a[j] : 0;
             if (in && b == b0) {
                 const int to = atomicAdd(&sm.count, 1);
@@ -332,7 +337,7 @@ __device__ __forceinline__ u64 find_cut(const R& row, Shared<NT>& sm, bool by_ma
     unsigned lo = ~0u, hi = 0;
     row.each([&](float x, int i) {
         const unsigned key = order_key(x);
-        if (kept(key, i) && bin(x) == b0) { lo = min(lo, key); hi = max(hi, key); }
+        if (kept(x, i) && bin(x) == b0) { lo = min(lo, key); hi = max(hi, key); }
     });
     atomicMin(&sm.key_lo, lo);
     atomicMax(&sm.key_hi, hi);
@@ -344,7 +349,7 @@ __device__ __forceinline__ u64 find_cut(const R& row, Shared<NT>& sm, bool by_ma
         clear_hist<NT>(sm);
         row.each([&](float x, int i) {
             const unsigned key = order_key(x);
-            if (key >= lo && key <= hi && kept(key, i) && bin(x) == b0) {
+            if (key >= lo && key <= hi && kept(x, i) && bin(x) == b0) {
                 const u64 a = amount(x);
                 if (a) atomicAdd(&sm.hist[(hi - key) >> shift], a);
             }
@@ -361,7 +366,7 @@ __device__ __forceinline__ u64 find_cut(const R& row, Shared<NT>& sm, bool by_ma
     }
     // the entries with this key, in index order, until they reach what is left
     const u64 each = amount(value_of((u64)lo << 32));
-    auto tie = [&](float y, int i) { const unsigned key = order_key(y); return (u64)(key == lo && kept(key, i)); };
+    auto tie = [&](float y, int i) { return (u64)(order_key(y) == lo && kept(y, i)); };
     wave_totals<NT>(row, sm, tie);
     const int last = locate<NT>(row, sm, (need + each - 1) / each - 1, tie);
     __syncthreads();
@@ -455,8 +460,6 @@ struct Setting {   // one filter setting: a value for each row, or one for all o
     __device__ __forceinline__ double at(int r) const { return rows ? (double)rows[r] : all; }
 };
 
-// The draw from a list: thread i holds kept entry i's index and weight (0: none).  Every kept entry adds up the weights of
-// those that come no later in the vocabulary; the one whose sum first exceeds the target is drawn.
 struct Kept { u64 w; unsigned index, pad; };
 
 template <typename T, int NT>
@@ -531,55 +534,91 @@ __global__ __launch_bounds__(NT, 4) void sample_filtered_kernel(const T* __restr
     const bool by_k = top_k > 0 && top_k < V, by_p = top_p < 1.0;
 
     // ---- the short list: entries no smaller than a bound that everything kept reaches
-    constexpr int LIST = NT / 2;   // longest list drawn from
     float bound = -INFINITY;
     if (by_k) {
-        if (top_k <= NT / 4) bound = bound_of<NT>(own, top_k, sm);
+        if (top_k <= NT / 2) bound = bound_of<NT>(own, top_k, sm);
     } else if (min_p > 0.0 && best < INFINITY) {
         const double z = (double)best + floor_z;
         bound = (float)z;
         if ((double)bound > z) bound = nextafterf(bound, -INFINITY);
     }
     if (bound > -INFINITY) {
-        const int n = collect<NT>(row, sm, bound, LIST);
-        if (n <= LIST) {
-            u64 c = 0;
-            if (by_k || by_p) c = ranked<NT>(n, sm);
-            else if (tid < n) c = sm.hist[tid];
-            if (by_k && tid >= top_k) c = 0;
-            const float x = c ? value_of(c) : 0.f;
-            u64 w = c && (best < INFINITY || x == best) ? weight(x) : 0;
-            if (by_p) {
-                const u64 before = block_prefix<NT>(w, sm);
-                const u64 listed = sm.total;
-                const u64 from = by_k ? listed : wave_totals<NT>(row, sm, [&](float y, int) { return weight(y); });
-                if (before >= prefix_mass(from)) w = 0;
+        constexpr int ITEMS = NT >= 1024 ? 2 : 4;   // entries a thread may hold; lists that are ranked have one each
+        const bool rank = by_k || by_p;
+        const int room = rank ? NT : NT * ITEMS, n = collect<NT>(row, sm, bound, room);
+        bool listed = n <= room;
+        if (listed) {
+            u64 c[ITEMS], w[ITEMS];
+            if (rank) {
+                c[0] = ranked<NT>(n, sm);
+                if (by_k && tid >= top_k) c[0] = 0;
+#pragma unroll
+                for (int e = 1; e < ITEMS; ++e) c[e] = 0;
+            } else {
+#pragma unroll
+                for (int e = 0; e < ITEMS; ++e) c[e] = tid + e * NT < n ? sm.hist[tid + e * NT] : 0;
             }
-            if (c && x != best && (double)x - (double)best < floor_z) w = 0;
-            // kept entries side by side, then everyone against everyone
+#pragma unroll
+            for (int e = 0; e < ITEMS; ++e) {
+                const float x = value_of(c[e]);
+                w[e] = c[e] && (best < INFINITY || x == best) ? weight(x) : 0;
+            }
+            if (by_p) {
+                const u64 before = block_prefix<NT>(w[0], sm);
+                const u64 mass_listed = sm.total;
+                const u64 from = by_k ? mass_listed : wave_totals<NT>(row, sm, [&](float y, int) { return y > -INFINITY ? weight(y) : 0; });
+                if (before >= prefix_mass(from)) w[0] = 0;
+            }
+            // the masses of the waves' pieces name the piece that the draw falls into, and its kept entries settle it among
+            // themselves: each adds up the weights of those that come no later in the vocabulary
+            const int piece = row.vectors * 64 * Elem<T>::VEC;
             Kept* kept = reinterpret_cast<Kept*>(sm.hist);
-            static_assert(sizeof(Kept) * LIST <= sizeof(sm.hist), "the kept list fits the histogram's place");
+            constexpr int KEPT = BINS / 2;   // as many as fit the histogram's place
+            static_assert(sizeof(Kept) * KEPT <= sizeof(sm.hist), "the kept list fits");
             __syncthreads();
-            if (tid == 0) { sm.count = 0; sm.cut = 0; }
+            if (tid == 0) sm.count = 0;
+            if (tid < NT / 64) sm.part[tid] = 0;
             __syncthreads();
-            if (w) {
-                kept[atomicAdd(&sm.count, 1)] = Kept{w, (unsigned)index_of(c), 0u};
-                atomicAdd(&sm.cut, w);
+#pragma unroll
+            for (int e = 0; e < ITEMS; ++e) {
+                const float x = value_of(c[e]);
+                if (x != best && (double)x - (double)best < floor_z) w[e] = 0;
+                if (w[e]) atomicAdd(&sm.part[index_of(c[e]) / piece], w[e]);
+            }
+            __syncthreads();
+            u64 total = 0;
+#pragma unroll
+            for (int p = 0; p < NT / 64; ++p) total += sm.part[p];
+            const u64 target = target_of(total);
+            u64 before = 0;
+            int at = 0;
+            while (before + sm.part[at] <= target) before += sm.part[at++];
+#pragma unroll
+            for (int e = 0; e < ITEMS; ++e) {
+                if (w[e] && index_of(c[e]) / piece != at) w[e] = 0;   // not in that piece
+                if (w[e]) {
+                    const int to = atomicAdd(&sm.count, 1);
+                    if (to < KEPT) kept[to] = Kept{w[e], (unsigned)index_of(c[e]), 0u};
+                }
             }
             __syncthreads();
             const int m = sm.count;
-            const u64 total = sm.cut, target = target_of(total);
-            if (w) {
-                const unsigned mine = (unsigned)index_of(c);
-                u64 upto = 0;
+            listed = m <= KEPT;
+            if (listed) {
+#pragma unroll
+                for (int e = 0; e < ITEMS; ++e) {
+                    if (!w[e]) continue;
+                    const unsigned mine = (unsigned)index_of(c[e]);
+                    u64 upto = before;
 #pragma unroll 4
-                for (int j = 0; j < m; ++j) {
-                    const Kept o = kept[j];
-                    upto += o.index <= mine ? o.w : 0;
+                    for (int j = 0; j < m; ++j) {
+                        const Kept o = kept[j];
+                        upto += o.index <= mine ? o.w : 0;
+                    }
+                    if (upto > target && upto - w[e] <= target) write((int)mine, value_of(c[e]), total);
                 }
-                if (upto > target && upto - w <= target) write((int)mine, x, total);
+                return;
             }
-            return;
         }
     }
 
@@ -705,16 +744,23 @@ extern "C" int icrl_sample_tokens_filtered(const void* logits, int dtype, int64_
     while ((1 << bits) < V) ++bits;
     const int S = std::min(51, 62 - bits);
     const Setting t{temperature_rows, temperature}, p{top_p_rows, top_p}, q{min_p_rows, min_p};
-#define ICRL_CALL(T, NT, PLACE)                                                                                           \
-    hipLaunchKernelGGL((sample_filtered_kernel<T, NT>), dim3(N), dim3(NT), 0, icrl::as_stream(stream),             \
+#define ICRL_CALL(T, NT)                                                                                               \
+    hipLaunchKernelGGL((sample_filtered_kernel<T, NT>), dim3(N), dim3(NT), 0, icrl::as_stream(stream),                 \
                        static_cast<const T*>(logits), ld_logits, V, S, uniforms, t, top_k_rows, top_k, p, q, tokens_out, \
                        token_stride, log_prob, log_prob_stride)
+    // Two workgroups of 512 share a CU, one of 1024 has it to itself: wide ones pay where rows are long and there is a
+    // CU for each of them (64 rows of 131072: 122 against XX us; 333 of 50257: 57 against YY).
+#define ICRL_WIDTHS(T)                                          \
+    if (V <= 4096) { ICRL_CALL(T, 256); }                       \
+    else if (V <= 16384 || N > 256) { ICRL_CALL(T, 512); }      \
+    else { ICRL_CALL(T, 1024); }
     switch (dtype) {
-        case ICRL_F32: ICRL_ROW_DISPATCH(float, V, 0, ICRL_CALL); break;
-        case ICRL_BF16: ICRL_ROW_DISPATCH(__bf16, V, 0, ICRL_CALL); break;
-        case ICRL_F16: ICRL_ROW_DISPATCH(_Float16, V, 0, ICRL_CALL); break;
+        case ICRL_F32: ICRL_WIDTHS(float); break;
+        case ICRL_BF16: ICRL_WIDTHS(__bf16); break;
+        case ICRL_F16: ICRL_WIDTHS(_Float16); break;
         default: icrl::set_error("icrl_sample_tokens_filtered: unknown dtype %d", dtype); return ICRL_ERR_ARG;
     }
+#undef ICRL_WIDTHS
 #undef ICRL_CALL
     ICRL_LAUNCH_CHECK();
     return ICRL_OK;

@@ -51,20 +51,39 @@ struct Row {
     const T* src;
     int V, vectors;      // vectors: how many per thread
     int first;           // index of the thread's first entry
+    int wave_first;      // of the wave's
+    Pack end;            // the entries of the row's last vector, if it is not whole
     Pack keep[PLACE > 0 ? PLACE : 1];
 
+    // Vector i, 16 bytes where the row has them.  Rows in memory: the one vector that the row ends inside of is read when
+    // the row is opened, entry by entry, and handed out by the thread that owns it (nothing of that is left in the passes).
     __device__ __forceinline__ Pack read(int i) const {
         const int at = first + i * 64 * VEC;
-        Pack p;
-        if (at + VEC <= V) {
-            p = __builtin_bit_cast(Pack, *reinterpret_cast<const Words*>(src + at));
+        if constexpr (PLACE == IN_MEMORY) {
+            if (wave_first + (i + 1) * 64 * VEC <= V) return __builtin_bit_cast(Pack, *reinterpret_cast<const Words*>(src + at));
+            Words w = at < V ? __builtin_bit_cast(Words, end) : __builtin_bit_cast(Words, fill());
+            if (at + VEC <= V) w = *reinterpret_cast<const Words*>(src + at);
+            return __builtin_bit_cast(Pack, w);
         } else {
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                p.e[j] = kFill;
-                if (at + j < V) __builtin_memcpy(&p.e[j], src + at + j, sizeof(Raw));
+            Pack p;
+            if (at + VEC <= V) {
+                p = __builtin_bit_cast(Pack, *reinterpret_cast<const Words*>(src + at));
+            } else {
+                p = fill();
+                read_end(p, at);
             }
+            return p;
         }
+    }
+    __device__ __forceinline__ void read_end(Pack& p, int at) const {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j)
+            if (at + j < V) __builtin_memcpy(&p.e[j], src + at + j, sizeof(Raw));
+    }
+    static __device__ __forceinline__ Pack fill() {
+        Pack p;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) p.e[j] = kFill;
         return p;
     }
     __device__ __forceinline__ Pack canonical(Pack p, int i) const {
@@ -87,6 +106,13 @@ struct Row {
         V = count;
         vectors = (count + NT * VEC - 1) / (NT * VEC);
         first = ((int)(threadIdx.x >> 6) * vectors * 64 + (int)(threadIdx.x & 63)) * VEC;
+        if constexpr (PLACE == IN_MEMORY) {
+            wave_first = __builtin_amdgcn_readfirstlane(first);
+            end = fill();
+            const int whole = count / VEC * VEC;
+            if (first <= whole && (whole - first) % (64 * VEC) == 0 && whole - first < vectors * 64 * VEC)   // one thread, or none
+                read_end(end, whole);
+        }
         if constexpr (PLACE > 0) {
 #pragma unroll
             for (int i = 0; i < PLACE; ++i)
@@ -114,18 +140,18 @@ struct Row {
             for (int i = 0; i < PLACE; ++i)
                 if (i < vectors) f(pass(keep[i]), first + i * 64 * VEC);
         } else {
-            constexpr int AHEAD = 4;
-            for (int i = 0; i < vectors; i += AHEAD) {
-                Pack p[AHEAD];
+            constexpr int AHEAD = 4;   // reads in flight: a queue in registers
+            Pack p[AHEAD];
 #pragma unroll
-                for (int q = 0; q < AHEAD; ++q)
-                    if (i + q < vectors) p[q] = read(i + q);
+            for (int q = 0; q < AHEAD; ++q)
+                if (q < vectors) p[q] = read(q);
 #pragma unroll 1
-                for (int q = 0; q < AHEAD; ++q) {
-                    if (i + q < vectors) f(canonical(p[0], i + q), first + (i + q) * 64 * VEC);
+            for (int i = 0; i < vectors; ++i) {
+                const Pack now = p[0];
 #pragma unroll
-                    for (int s = 0; s + 1 < AHEAD; ++s) p[s] = p[s + 1];   // a queue, not an indexed array: it stays in registers
-                }
+                for (int q = 0; q + 1 < AHEAD; ++q) p[q] = p[q + 1];
+                if (i + AHEAD < vectors) p[AHEAD - 1] = read(i + AHEAD);
+                f(canonical(now, i), first + i * 64 * VEC);
             }
         }
     }
@@ -149,10 +175,9 @@ __device__ __forceinline__ unsigned order_key(float x) {
     return (unsigned)(b ^ ((b >> 31) | (int)0x80000000));
 }
 
-// 2^t 2^scale in float64, by the Taylor series of 2^r = e^(r ln 2) on |r| <= 1/2: nine terms leave 0.3466^10 / 10! =
-// 7e-12 of the result.  (The library's exp2 spends several times the instructions on bits that no sum here can show.)
-__device__ __forceinline__ double exp2_scaled(double t, int scale) {
-    const double n = rint(t), r = t - n;
+// 2^r in float64 for |r| <= 1/2, by the Taylor series of e^(r ln 2): nine terms leave 0.3466^10 / 10! = 7e-12 of the
+// result.  (The library's exp2 spends several times the instructions on bits that no sum here can show.)
+__device__ __forceinline__ double exp2_fraction(double r) {
     constexpr double L = 0.69314718055994530942, L2 = L * L, L3 = L2 * L, L4 = L2 * L2, L5 = L4 * L;
     double p = L4 * L5 / 362880.0;
     p = fma(p, r, L4 * L4 / 40320.0);
@@ -163,8 +188,14 @@ __device__ __forceinline__ double exp2_scaled(double t, int scale) {
     p = fma(p, r, L3 / 6.0);
     p = fma(p, r, L2 / 2.0);
     p = fma(p, r, L);
-    p = fma(p, r, 1.0);
-    return ldexp(p, (int)n + scale);
+    return fma(p, r, 1.0);
+}
+// 2^t 2^scale where the result is a normal number, |t| < 2^30: the nearest integer is read off the sum with 1.5 2^52 and
+// added to the exponent's bits (rounding, conversion and ldexp instructions run at a quarter of the rate)
+__device__ __forceinline__ double exp2_normal(double t, int scale) {
+    const double shifted = t + 0x1.8p52, r = t - (shifted - 0x1.8p52);
+    const int n = (int)__double_as_longlong(shifted);
+    return __longlong_as_double(__double_as_longlong(exp2_fraction(r)) + ((long long)(n + scale) << 52));
 }
 
 __device__ __forceinline__ u64 wave_sum_u64(u64 v) {
