@@ -819,6 +819,43 @@ class A2CEngine:
         self._policy_backward(ws, features, n, 1, s)
         return ws["scalars"][0:1]
 
+    def policy_distill_step(self, features, captions, record, row_weight, temperature=1.0):
+        """policy_ce_step with a teacher in place of the captions' next words: captions [N, L] int64 cuda are walked
+        teacher-forced, and the student's distribution at each of the (L - 1) N positions (position by position) is drawn
+        to the one that record = (values [rows, k], indices [rows, k], log-normaliser [rows] or None) describes
+        (hipabi.distill_loss).  row_weight [L - 1, N]; positions of weight 0 are left out.  Fills the policy gradients;
+        returns the loss, the sum over the positions, as a 1-element device tensor."""
+        P = self.P
+        n, l_cols = captions.shape
+        s = l_cols - 1
+        values, indices, lse = record
+        assert values.shape[0] == s * n and row_weight.shape == (s, n)
+        ws = self._buffers(n, 1, s)
+        # an A2C step on the same shape shares this workspace: none of its pending work belongs to this pass
+        ws["policy_early"] = False
+        for key in ("early_pending", "head_grads_pending", "h0_done", "cell0_done"):
+            ws.pop(key, None)
+        self._forget_scales(ws)
+        ws["tokT"].copy_(captions.t())
+        self._rollout_h0(ws, features)
+        ws["rollout_id"] = ws.get("rollout_id", 0) + 1   # (what is derived from ws["dlogits"] is kept under it)
+        for k in range(s):
+            self._rollout_cell(ws, k, n, self.E % 64 == 0 and self.pd == "f32")
+        ws["X_pending"] = False
+        # all positions' logits in one product, and their gradient in the logits' place: 0.4 GB less to hold and to write
+        G0 = ws["dlogits"].view(s * n, self.vocab)
+        hip.gemm(ws["Hbuf"][1:].view(s * n, H), P["linear2vocab.weight"], G0, bias=P["linear2vocab.bias"], dtype=self.pd)
+        self._order_tokens(ws, n, s * n, torch.cuda.current_stream(), torch.cuda.current_stream())
+        hip.distill_loss(G0, values, indices, ws["logp"].view(-1), teacher_lse=lse, temperature=temperature,
+                         row_weight=row_weight.reshape(-1).contiguous(), dlogits=G0)
+        hip.colsum(ws["logp"].view(-1, 1), ws["scalars"][0:1], scratch=ws["cs_main"])
+        ws["dlogp"].fill_(1.0)
+        # (the rows are no onehot - softmax, whose largest entry the log-probabilities tell: their scales take a pass)
+        self._pgemm(ws, "uvoc", G0, P["linear2vocab.weight"], ws["Uvocab"], ws["scratch_side"], self.vgd, b_kmajor=True,
+                    shared=True)
+        self._policy_backward(ws, features, n, 1, s, uvocab_done=True)
+        return ws["scalars"][0:1]
+
     def value_mse_step(self, features, captions, targets):
         """Mean-squared-error step of the value pre-training loop (trainers.py:175-190): one
         ValueNetwork call on captions [N, p] (its batch-1 chain walked exactly), nn.MSELoss against
@@ -1890,13 +1927,13 @@ class A2CEngine:
         if ev_side is not None:
             main.wait_event(ev_side)
 
-    def _policy_backward(self, ws, features, n, p0, s):
+    def _policy_backward(self, ws, features, n, p0, s, uvocab_done=False):
         """Backward of the policy network from ws["dlogp"] = dLoss/dlog_prob (one coefficient per (step, row)).
         d logits = coef * G0 with G0 = onehot - softmax, so the coefficient is applied to small matrices instead
         of the [rows, V] one: what flows into the LSTM outputs is coef * (G0 . W) (G0 . W formed before the loss
         when _policy_backward_early ran), the vocabulary matrix's gradient is G0^T . (coef * Hs) and its bias
         gradient sum_r coef[r] G0[r, :].  The two vocabulary-sized gradients run on the third stream beside the
-        LSTM's backward-through-time."""
+        LSTM's backward-through-time.  uvocab_done: the caller has formed ws["Uvocab"] (with G0 of its own making)."""
         P, gP = self.P, self.gP
         t_steps = p0 - 1 + s
         coef = ws["dlogp"]
@@ -1906,7 +1943,7 @@ class A2CEngine:
         cur = torch.cuda.current_stream()
         if ws.get("policy_early"):
             cur.wait_event(ws["ev_early"])
-        else:
+        elif not uvocab_done:
             self._uvocab(ws, G0, ss)
         dHall = ws["dHall"]
         if p0 > 1:

@@ -113,6 +113,15 @@ class PolicyNetwork(nn.Module):
         hip.gemm(hs[1:].view(p * n, H), self.linear2vocab.weight, logits, bias=self.linear2vocab.bias)
         return logits.view(p, n, vocab).permute(1, 0, 2)
 
+    @torch.no_grad()
+    def vocab_weight8(self):
+        """The vocabulary matrix cut to 8 bits (hipabi.cut_fp8: e4m3, a power-of-two scale per word and block of 128),
+        for decoding: GenerateCaptionsSampled(vocab8=...).  Of the weights as they are now: cut again after training."""
+        w = self.linear2vocab.weight
+        pieces = hip.fp8_pieces(w.shape[0], w.shape[1], w.device)
+        hip.cut_fp8(w, *pieces)
+        return pieces
+
 
 class ValueNetworkRNN(nn.Module):
     """Embedding + LSTM fed (N,1,E) without batch_first: the rows of a minibatch are

@@ -91,6 +91,60 @@ def GenerateCaptionsGreedy(features, captions, policy_network):
 
 
 @torch.no_grad()
+def GenerateCaptionsSampled(features, captions, policy_network, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
+                            uniforms=None, vocab8=None):
+    """GenerateCaptionsGreedy with every word drawn from the filtered and tempered distribution
+    (hipabi.sample_tokens_filtered; the reference decodes greedily or samples the plain softmax, trainers.py:57-70,
+    444-458): MAX_SEQ_LEN - 1 steps from captions[:, 0:1] -> ([N, 17] int64, log-probabilities [N, 16] of the drawn
+    words).  Each setting is a number or an [N] tensor.  uniforms [16, N] float64 (default: NumPy's global stream, one
+    double per step and row, as the training rollout draws).  vocab8: policy_network.vocab_weight8(), to form the logits
+    from the 8-bit vocabulary matrix (the state keeps its float32 products)."""
+    w = policy_network.cnn2linear.weight
+    dev = w.device
+    feats = torch.as_tensor(features, device=dev).float().contiguous()
+    caps = torch.as_tensor(np.asarray(captions)[:, 0:1] if not torch.is_tensor(captions) else captions[:, 0:1],
+                           device=dev).long()
+    n, steps = feats.shape[0], MAX_SEQ_LEN - 1
+    vocab = policy_network.linear2vocab.weight.shape[0]
+    if uniforms is None:
+        uniforms = torch.from_numpy(np.random.random_sample((steps, n)))
+    uniforms = torch.as_tensor(uniforms, dtype=torch.float64, device=dev).contiguous()
+    assert uniforms.shape == (steps, n), "uniforms must be [%d, %d]" % (steps, n)
+    tok_t = torch.zeros(MAX_SEQ_LEN, n, dtype=torch.int64, device=dev)
+    tok_t[0] = caps[:, 0]
+    log_prob = torch.empty(steps, n, device=dev)
+    h = torch.empty(n, H, device=dev)
+    c_prev, c_next = torch.zeros(n, H, device=dev), torch.empty(n, H, device=dev)
+    gates, logits = torch.empty(n, 4 * H, device=dev), torch.empty(n, vocab, device=dev)
+    h8 = None if vocab8 is None else hip.fp8_pieces(n, H, dev)
+    failed = torch.zeros(n, dtype=torch.bool, device=dev)
+    lstm, linear = policy_network.lstm, policy_network.linear2vocab
+    hip.gemm(feats, w, h, bias=policy_network.cnn2linear.bias)
+    for t in range(steps):
+        hip.gemm(policy_network.caption_embedding.weight, lstm.weight_ih_l0, gates, a_rows=tok_t[t],
+                 bias=lstm.bias_ih_l0, bias2=lstm.bias_hh_l0)
+        hip.gemm(h, lstm.weight_hh_l0, gates, accumulate=True)
+        hip.lstm_cell_fwd(gates, c_prev, c_next, h)
+        c_prev, c_next = c_next, c_prev
+        if vocab8 is None:
+            hip.gemm(h, linear.weight, logits, bias=linear.bias)
+        else:
+            hip.cut_fp8(h, *h8)
+            hip.gemm_fp8(*h8, *vocab8, logits, H, bias=linear.bias)
+        hip.sample_tokens_filtered(logits, tok_t[t + 1], 1, uniforms[t], temperature=temperature, top_k=top_k, top_p=top_p,
+                                   min_p=min_p, log_prob=log_prob[t])
+        if t + 1 < steps:
+            # a row that draws nothing (token -1) goes on from word 0, and is reported at the end
+            failed |= tok_t[t + 1] < 0
+            tok_t[t + 1].clamp_(min=0)
+    failed |= tok_t[steps] < 0
+    if bool(failed.any()):
+        raise RuntimeError("row %d drew no word: its logits hold a NaN, or its settings are out of range"
+                           % int(failed.nonzero()[0]))
+    return tok_t.t().contiguous(), log_prob.t().contiguous()
+
+
+@torch.no_grad()
 def GenerateCaptionsWithActorCriticLookAhead(features, captions, policy_network, value_network, beamSize=5,
                                              most_likely=False):
     """Beam look-ahead decoding (trainers.py:73-105): every step each kept candidate is extended by the
@@ -350,6 +404,57 @@ def train_policy_network(train_data, network_paths, plot_dir, bidirectional, epo
             optimizer.step()
     _after_checkpoints()
     return policy_network
+
+
+@torch.no_grad()
+def teacher_record(policy_network, features, captions, top=64, temperature=1.0):
+    """What a trained policy network leaves for a student: for every teacher-forced position of captions [N, L] its `top`
+    largest logits (values, word indices: [(L - 1) N, top], position by position) and the log-normaliser of the whole
+    row at `temperature` [(L - 1) N]."""
+    caps = torch.as_tensor(np.asarray(captions) if not torch.is_tensor(captions) else captions)
+    logits = policy_network(torch.as_tensor(features).unsqueeze(0), caps[:, :-1])       # [N, L - 1, V], stored [L - 1, N, V]
+    rows = logits.permute(1, 0, 2).reshape(-1, logits.shape[2])
+    values = torch.empty(rows.shape[0], top, device=rows.device)
+    indices = torch.empty(rows.shape[0], top, dtype=torch.int64, device=rows.device)
+    lse = torch.empty(rows.shape[0], device=rows.device)
+    hip.topk_lse_rows(rows, values, indices, lse, temperature=temperature)
+    return values, indices, lse
+
+
+def distill_policy_network(train_data, teacher_network, network_paths, plot_dir, epochs=100, batch_size=512, top=64,
+                           temperature=2.0, student_network=None):
+    """train_policy_network with a teacher in place of the captions' next words (no counterpart in the reference): the
+    student's distribution at every teacher-forced position is drawn to the teacher's, known by its `top` largest
+    logits, at `temperature`; positions and rows weigh what they weigh there (trainers.py:238-242), times temperature
+    squared, which keeps the gradients' size.  Adam(lr=1e-3); the parameters are saved to
+    network_paths["policy_network"] whenever a minibatch improves on the best loss seen."""
+    fdim = int(np.asarray(train_data["train_features"]).shape[1])
+    if student_network is None:
+        student_network = PolicyNetwork(train_data["word_to_idx"], input_dim=fdim,
+                                        pretrained_embeddings=train_data["embeddings"]).to(device)
+    flat = flatten_module(student_network)
+    ddp.broadcast_parameters(flat.flat)
+    optimizer = FusedAdam(flat, lr=0.001)
+    engine = A2CEngine(_params_of(student_network), None, None, _grads_of(student_network))
+    writer = make_writer(plot_dir)
+    best_loss = float("inf")
+    print_green('[Training] Distilling Policy Network')
+    for epoch in range(epochs):
+        for minibatch_id, (captions, features, _) in enumerate(
+                minibatches(train_data, batch_size=batch_size, split='train')):
+            caps = torch.as_tensor(np.asarray(captions), device=device).long().contiguous()
+            feats = torch.as_tensor(features, device=device).float().contiguous()
+            steps = caps.shape[1] - 1
+            valid, weight = _ce_weights(captions, steps)
+            weights = weight[None, :] * temperature ** 2 * (np.arange(steps)[:, None] < valid[None, :])
+            loss = engine.policy_distill_step(feats, caps, teacher_record(teacher_network, feats, caps, top, temperature),
+                                              torch.from_numpy(weights.astype(np.float32)).to(device), temperature).item()
+            best_loss = _save_if_best(loss, best_loss, student_network, network_paths["policy_network"])
+            writer.add_scalar('Policy Network-distillation-loss', loss, global_minibatch_number(epoch, minibatch_id, batch_size))
+            ddp.average_gradients(flat.flat_grad)
+            optimizer.step()
+    _after_checkpoints()
+    return student_network
 
 
 def train_value_network(train_data, network_paths, plot_dir, bidirectional, epochs=50, batch_size=512):

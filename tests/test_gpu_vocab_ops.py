@@ -555,3 +555,19 @@ def test_bindings_refuse_what_does_not_fit():
         hip.cut_fp8(torch.zeros(40, 100, device="cuda"), pieces, scales)
     with pytest.raises(AssertionError):
         hip.gemm_fp8(pieces, scales, pieces, scales, torch.empty(4, 4, device="cuda"), 1000)
+
+
+@pytest.mark.parametrize("kept", [200, 700, 1500, 3000, 9000])
+def test_sampling_lists_of_every_length(kept):
+    """min-p keeps `kept` words: within a thread's entries, more than that, and more than the lists hold."""
+    v = 30000
+    for dtype in (F32, BF16):
+        x = torch.full((4, v), -3.0, dtype=dtype, device="cuda")
+        where = torch.randperm(v, generator=torch.Generator().manual_seed(kept))[:kept].cuda()
+        x[:, where] = (torch.rand(kept, generator=torch.Generator().manual_seed(1)) * 2.0).to(dtype).cuda()
+        x[3, :] = -30.0
+        x[3, 5000:5000 + kept] = 1.0      # all of them in one wave's piece, or two
+        u = np.array([0.0, 0.37, 0.999, 0.61])
+        for s in (dict(min_p=0.1), dict(min_p=0.1, top_p=0.8), dict(top_k=kept), dict(top_k=kept, top_p=0.5, min_p=0.2)):
+            tokens, lp = draw(x, u, **s)
+            check_draw(x, u, s, tokens, lp)
