@@ -241,11 +241,21 @@ __device__ __forceinline__ u64 ranked(int n, Shared<NT>& sm) {
     return block_sort<NT>(c, sm.hist);
 }
 
+// Equal value ranges counted from the top: monotone in the row's order; what is far below the top, NaN included, is the
+// last one, and +inf, which lies above a finite top, the first.
+struct RangeBins {
+    float top, per;
+    __device__ __forceinline__ int operator()(float x) const {
+        const float at = (top - x) * per;
+        return at < (float)(BINS - 1) ? (int)fmaxf(at, 0.f) : BINS - 1;
+    }
+};
+
 // The cut after the shortest prefix (in the row's order, among the entries with composite >= `from`) whose amounts -
 // by_mass: weights, else 1 each - reach need_of(total).  width: the value range that the first histogram spreads over its
 // bins, counted from the top; any positive width gives the same cut, a good one makes the second step short.
 // Weights are computed for a whole vector before anything depends on one of them: a weight is a chain of some 20 float64
-// instructions, and only side by side do they hide each other's latency (400 clocks an entry otherwise, 100 so).
+// instructions, and only side by side do they hide each other's latency.
 // Returns with the kept masses of the waves' pieces in sm.part and their total in `mass_kept` if by_mass and the second
 // step was the short one; otherwise mass_kept is 0.
 template <int NT, typename R, typename G>
@@ -260,11 +270,7 @@ __device__ __forceinline__ u64 find_cut(const R& row, Shared<NT>& sm, bool by_ma
         return whole ? i < row.V : (x > from_x) | ((x == from_x) & ((unsigned)i <= from_index));
     };
     auto amount = [&](float x) { return by_mass ? weight(x) : (u64)1; };
-    const float per = (float)BINS / width, top = (float)weight.top;
-    auto bin = [&](float x) {   // monotone in the row's order; what is far below the top, NaN included, is the last bin
-        const float at = (top - x) * per;
-        return at < (float)(BINS - 1) ? (int)fmaxf(at, 0.f) : BINS - 1;   // (+inf lies above a finite top: bin 0)
-    };
+    const RangeBins bin{(float)weight.top, (float)BINS / width};
     auto amounts = [&](const typename R::Pack& p, u64 (&a)[VEC]) {
         if (by_mass) {
 #pragma unroll
@@ -460,24 +466,108 @@ struct Setting {   // one filter setting: a value for each row, or one for all o
     __device__ __forceinline__ double at(int r) const { return rows ? (double)rows[r] : all; }
 };
 
+struct Requests {
+    const double* uniforms;
+    Setting temperature, top_p, min_p;
+    const int* top_k_rows;
+    int top_k_all;
+};
+struct Results {
+    int64_t* tokens;
+    int64_t token_stride;
+    float* log_prob;
+    int64_t lp_stride;
+};
+
+// One row's settings, and what follows from them.
+struct Request {
+    double temp, top_p, min_p, u, floor_z;   // w >= min_p as x - best >= floor_z = T log(min_p)
+    int top_k;
+    __device__ __forceinline__ Request(const Requests& all, int r)
+        : temp(all.temperature.at(r)), top_p(all.top_p.at(r)), min_p(all.min_p.at(r)), u(all.uniforms[r]), floor_z(-INFINITY),
+          top_k(all.top_k_rows ? all.top_k_rows[r] : all.top_k_all) {
+        if (min_p > 0.0) floor_z = log(min_p) * temp;
+    }
+    __device__ __forceinline__ bool fine() const {
+        return temp >= 0.0 && temp < INFINITY && top_k >= 0 && top_p >= 0.0 && top_p <= 1.0 && min_p >= 0.0 && min_p <= 1.0 && u == u;
+    }
+    __device__ __forceinline__ u64 prefix_mass(u64 total) const {   // what top_p asks for
+        const double w = ceil(top_p * (double)total);
+        const u64 want = w < 1.0 ? 1 : (u64)w;
+        return want < total ? want : total;
+    }
+    __device__ __forceinline__ u64 target(u64 total) const {
+        const double want = u * (double)total;
+        const u64 t = want > 0.0 ? (u64)fmin(want, 0x1p63) : 0;
+        return t < total ? t : total - 1;
+    }
+    // value range that holds every entry with weight: entries further below the top have none
+    __device__ __forceinline__ float reach(int S) const { return fmaxf((float)(S * 0.6931471805599453 * temp), 1e-30f); }
+    // value range below which lies less than e^-7 of the top's weight, V entries taken together: up to top_p = 0.999 no
+    // cut lies there, and the bins over it are half as wide
+    __device__ __forceinline__ float span(int V, int S) const {
+        return fmaxf(fminf((float)temp * (__logf((float)V) + 7.f), reach(S)), 1e-30f);
+    }
+    __device__ __forceinline__ void write(const Results& out, int r, int token, float x, float best, u64 total, int S) const {
+        out.tokens[r * out.token_stride] = token;
+        if (out.log_prob) {
+            const double z = x == best ? 0.0 : ((double)x - (double)best) / temp;
+            out.log_prob[r * out.lp_stride] = (float)(z - log(ldexp((double)total, -S)));
+        }
+    }
+};
+
+// What of a row remains after the cut and min-p: the weight of entry i, value x, or 0.
+struct Mass {
+    Weights weight;
+    float best, cut_x;
+    unsigned cut_index;
+    double floor_z;
+    __device__ __forceinline__ u64 operator()(float x, int i) const {
+        const u64 w = weight(x);
+        const bool in = (x > cut_x) | ((x == cut_x) & ((unsigned)i <= cut_index));
+        const bool low = (x != best) & ((double)x - (double)best < floor_z);
+        return (in & !low) ? w : 0;
+    }
+};
+
+// Rows too long for one CU (split calls, see sample_chunk_mass): what the first launch leaves of a row, and where the
+// workgroups on its chunks meet.  8-byte words per row: the state, the pieces' masses, a list of entries, the histogram.
+struct RowState {
+    float best, per;    // per: bins per unit of value, computed once for both launches
+    int pending;        // 0: drawn; 1: top-p over the whole row; 2: no prefix to find
+    unsigned listed, ticket;
+};
+constexpr int CHUNK_NT = 512, MAX_PIECES = 512, ROOM = 512;
+constexpr int STATE_WORDS = 8, WORK_WORDS = STATE_WORDS + MAX_PIECES + ROOM + BINS;
+static_assert(ROOM <= CHUNK_NT && MAX_PIECES <= CHUNK_NT, "a thread ranks one entry and adds up one piece");
+struct Work {
+    u64* rows;
+    __device__ __forceinline__ RowState* state(int r) const { return reinterpret_cast<RowState*>(rows + (int64_t)r * WORK_WORDS); }
+    __device__ __forceinline__ u64* pieces(int r) const { return rows + (int64_t)r * WORK_WORDS + STATE_WORDS; }
+    __device__ __forceinline__ u64* list(int r) const { return pieces(r) + MAX_PIECES; }
+    __device__ __forceinline__ u64* hist(int r) const { return list(r) + ROOM; }
+};
+
 struct Kept { u64 w; unsigned index, pad; };
 
+// split.rows not null: rows that need the weights of all their entries are left to the launches that follow.
 template <typename T, int NT>
-__global__ __launch_bounds__(NT, 4) void sample_filtered_kernel(const T* __restrict__ logits, int64_t ld, int V, int S,
-                                                             const double* __restrict__ uniforms, Setting temperature,
-                                                             const int* __restrict__ top_k_rows, int top_k_all,
-                                                             Setting top_p_in, Setting min_p_in,
-                                                             int64_t* __restrict__ tokens, int64_t token_stride,
-                                                             float* __restrict__ log_prob, int64_t lp_stride) {
+__global__ __launch_bounds__(NT, 4) void sample_filtered_kernel(const T* __restrict__ logits, int64_t ld, int V, int S, Requests all,
+                                                                Results out, Work split) {
     __shared__ Shared<NT> sm;
     const int r = blockIdx.x, tid = threadIdx.x;
     // Read again by every pass: the passes that weigh entries, unrolled over a row in registers, would be far longer than
     // the instruction cache, and with registers to spare two workgroups fit a CU (512 rows of 10 000: 33 against 36 us)
     Row<T, NT, IN_MEMORY, false> row;
     row.open(logits + (int64_t)r * ld, V);
-    const double temp = temperature.at(r), top_p = top_p_in.at(r), min_p = min_p_in.at(r), u = uniforms[r];
-    const int top_k = top_k_rows ? top_k_rows[r] : top_k_all;
-    if (tid == 0) sm.flag = 0;
+    const Request q(all, r);
+    const int top_k = q.top_k;
+    const double floor_z = q.floor_z;
+    if (tid == 0) {
+        sm.flag = 0;
+        if (split.rows) split.state(r)->pending = 0;
+    }
     float best = -INFINITY;
     bool nan = false;
     row.each([&](float x, int) {
@@ -488,16 +578,14 @@ __global__ __launch_bounds__(NT, 4) void sample_filtered_kernel(const T* __restr
     best = block_max<NT>(best, sm.red);
     if (nan) sm.flag = 1;
     __syncthreads();
-    const bool fine = temp >= 0.0 && temp < INFINITY && top_k >= 0 && top_p >= 0.0 && top_p <= 1.0 && min_p >= 0.0 &&
-                      min_p <= 1.0 && u == u;
-    if (!fine || sm.flag || best == -INFINITY) {
+    if (!q.fine() || sm.flag || best == -INFINITY) {
         if (tid == 0) {
-            tokens[r * token_stride] = -1;
-            if (log_prob) log_prob[r * lp_stride] = NAN;
+            out.tokens[r * out.token_stride] = -1;
+            if (out.log_prob) out.log_prob[r * out.lp_stride] = NAN;
         }
         return;
     }
-    if (temp == 0.0 || top_k == 1 || top_p == 0.0) {   // the first largest entry
+    if (q.temp == 0.0 || top_k == 1 || q.top_p == 0.0) {   // the first largest entry
         if (tid == 0) sm.index = V;
         __syncthreads();
         if (own == best) {
@@ -507,37 +595,20 @@ __global__ __launch_bounds__(NT, 4) void sample_filtered_kernel(const T* __restr
         }
         __syncthreads();
         if (tid == 0) {
-            tokens[r * token_stride] = sm.index;
-            if (log_prob) log_prob[r * lp_stride] = 0.f;
+            out.tokens[r * out.token_stride] = sm.index;
+            if (out.log_prob) out.log_prob[r * out.lp_stride] = 0.f;
         }
         return;
     }
-    const Weights weight = weights_of(best, temp, S);
-    const double floor_z = min_p > 0.0 ? log(min_p) * temp : -INFINITY;   // w >= min_p as x - best >= T log(min_p)
-    auto write = [&](int token, float x, u64 total) {
-        tokens[r * token_stride] = token;
-        if (log_prob) {
-            const double z = x == best ? 0.0 : ((double)x - (double)best) / temp;
-            log_prob[r * lp_stride] = (float)(z - log(ldexp((double)total, -S)));
-        }
-    };
-    auto target_of = [&](u64 total) {
-        const double want = u * (double)total;
-        const u64 target = want > 0.0 ? (u64)fmin(want, 0x1p63) : 0;
-        return target < total ? target : total - 1;
-    };
-    auto prefix_mass = [&](u64 total) {   // what top_p asks for
-        const double w = ceil(top_p * (double)total);
-        const u64 want = w < 1.0 ? 1 : (u64)w;
-        return want < total ? want : total;
-    };
-    const bool by_k = top_k > 0 && top_k < V, by_p = top_p < 1.0;
+    const Weights weight = weights_of(best, q.temp, S);
+    const bool by_k = top_k > 0 && top_k < V, by_p = q.top_p < 1.0;
+    const bool leave = split.rows && !by_k;   // to the launches on the row's chunks, unless a list settles it
 
     // ---- the short list: entries no smaller than a bound that everything kept reaches
     float bound = -INFINITY;
     if (by_k) {
         if (top_k <= NT / 2) bound = bound_of<NT>(own, top_k, sm);
-    } else if (min_p > 0.0 && best < INFINITY) {
+    } else if (q.min_p > 0.0 && best < INFINITY && !(leave && by_p)) {
         const double z = (double)best + floor_z;
         bound = (float)z;
         if ((double)bound > z) bound = nextafterf(bound, -INFINITY);
@@ -567,7 +638,7 @@ __global__ __launch_bounds__(NT, 4) void sample_filtered_kernel(const T* __restr
                 const u64 before = block_prefix<NT>(w[0], sm);
                 const u64 mass_listed = sm.total;
                 const u64 from = by_k ? mass_listed : wave_totals<NT>(row, sm, [&](float y, int) { return y > -INFINITY ? weight(y) : 0; });
-                if (before >= prefix_mass(from)) w[0] = 0;
+                if (before >= q.prefix_mass(from)) w[0] = 0;
             }
             // the masses of the waves' pieces name the piece that the draw falls into, and its kept entries settle it among
             // themselves: each adds up the weights of those that come no later in the vocabulary
@@ -589,7 +660,7 @@ __global__ __launch_bounds__(NT, 4) void sample_filtered_kernel(const T* __restr
             u64 total = 0;
 #pragma unroll
             for (int p = 0; p < NT / 64; ++p) total += sm.part[p];
-            const u64 target = target_of(total);
+            const u64 target = q.target(total);
             u64 before = 0;
             int at = 0;
             while (before + sm.part[at] <= target) before += sm.part[at++];
@@ -615,22 +686,19 @@ __global__ __launch_bounds__(NT, 4) void sample_filtered_kernel(const T* __restr
                         const Kept o = kept[j];
                         upto += o.index <= mine ? o.w : 0;
                     }
-                    if (upto > target && upto - w[e] <= target) write((int)mine, value_of(c[e]), total);
+                    if (upto > target && upto - w[e] <= target) q.write(out, r, (int)mine, value_of(c[e]), best, total, S);
                 }
                 return;
             }
         }
     }
 
-    const float reach = fmaxf((float)(S * 0.6931471805599453 * temp), 1e-30f);   // entries further below weigh nothing
-    float cut_x = -INFINITY;
-    unsigned cut_index = 0;
-    auto mass = [&](float x, int i) -> u64 {
-        const u64 w = weight(x);
-        const bool in = (x > cut_x) | ((x == cut_x) & ((unsigned)i <= cut_index));
-        const bool low = (x != best) & ((double)x - (double)best < floor_z);
-        return (in & !low) ? w : 0;
-    };
+    if (leave) {
+        u64* hist = split.hist(r);
+        for (int b = tid; b < BINS; b += NT) hist[b] = 0;
+        if (tid == 0) *split.state(r) = RowState{best, (float)BINS / q.span(V, S), by_p ? 1 : 2, 0u, 0u};
+        return;
+    }
 
     // ---- the whole row
     // with an entry of +inf only the entries of +inf have weight (all the same)
@@ -639,14 +707,204 @@ __global__ __launch_bounds__(NT, 4) void sample_filtered_kernel(const T* __restr
         const bool by_mass = filter == 1;
         if (!(by_mass ? by_p : by_k)) continue;
         const u64 k = (u64)top_k;
-        cut = find_cut<NT>(row, sm, by_mass, cut, weight, reach, [&](u64 of) { return by_mass ? prefix_mass(of) : k < of ? k : of; },
-                           total);
+        cut = find_cut<NT>(row, sm, by_mass, cut, weight, by_mass ? q.span(V, S) : q.reach(S),
+                           [&](u64 of) { return by_mass ? q.prefix_mass(of) : k < of ? k : of; }, total);
     }
-    cut_x = value_of(cut);
-    cut_index = ~(unsigned)cut;
-    if (total == 0 || min_p > 0.0) total = wave_totals<NT>(row, sm, mass);
-    const int token = locate<NT>(row, sm, target_of(total), mass);
-    if (tid == 0) write(token, row.entry(token), total);
+    const Mass mass{weight, best, value_of(cut), ~(unsigned)cut, floor_z};
+    if (total == 0 || q.min_p > 0.0) total = wave_totals<NT>(row, sm, mass);
+    const int token = locate<NT>(row, sm, q.target(total), mass);
+    if (tid == 0) q.write(out, r, token, row.entry(token), best, total, S);
+}
+
+// ---- rows split over workgroups
+// A row's weights cost some 45 instructions an entry, twice (45 us a pass for 131072 entries on one CU), so where rows are
+// long and few their chunks are weighed side by side: one launch adds the chunks' histograms up (integers: any order
+// gives the same), the next collects the range of the cut and the masses above it, and the workgroup that finishes last
+// with a row draws.  No workgroup waits for another.
+template <typename T>
+__global__ __launch_bounds__(CHUNK_NT, 4) void sample_chunk_mass(const T* __restrict__ logits, int64_t ld, int V, int chunk, int S,
+                                                                 Requests all, Work split) {
+    constexpr int NT = CHUNK_NT;
+    __shared__ Shared<NT> sm;
+    const int r = blockIdx.y, tid = threadIdx.x, first = blockIdx.x * chunk;
+    const RowState state = *split.state(r);
+    if (state.pending != 1) return;
+    const Request q(all, r);
+    const Weights weight = weights_of(state.best, q.temp, S);
+    const RangeBins bin{(float)weight.top, state.per};
+    const float from = state.best == INFINITY ? INFINITY : -3.402823466e38f;
+    Row<T, NT, IN_MEMORY, false> row;
+    row.open(logits + (int64_t)r * ld + first, min(chunk, V - first));
+    clear_hist<NT>(sm);
+    u64 rest = 0;
+    row.each_pack([&](const auto& p, int) {
+        constexpr int VEC = Elem<T>::VEC;
+        u64 a[VEC];
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) a[j] = weight(Elem<T>::value(p.e[j]));
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            const float x = Elem<T>::value(p.e[j]);
+            const int b = bin(x);
+            rest += x >= from && b == BINS - 1 ? a[j] : 0;
+            if (x >= from && b < BINS - 1) atomicAdd(&sm.hist[b], a[j]);
+        }
+    });
+    rest = wave_sum_u64(rest);
+    if ((tid & 63) == 0 && rest) atomicAdd(&sm.hist[BINS - 1], rest);
+    __syncthreads();
+    u64* hist = split.hist(r);
+    for (int b = tid; b < BINS; b += NT)
+        if (sm.hist[b]) atomicAdd(&hist[b], sm.hist[b]);
+}
+
+template <typename T>
+__global__ __launch_bounds__(CHUNK_NT, 4) void sample_chunk_draw(const T* __restrict__ logits, int64_t ld, int V, int chunk, int S,
+                                                                 Requests all, Results out, Work split) {
+    constexpr int NT = CHUNK_NT, WAVES = NT / 64;
+    __shared__ Shared<NT> sm;
+    __shared__ u64 pieces[MAX_PIECES];
+    const int r = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, first = blockIdx.x * chunk;
+    const RowState state = *split.state(r);
+    if (state.pending == 0) return;
+    const Request q(all, r);
+    const float best = state.best;
+    const Weights weight = weights_of(best, q.temp, S);
+    const RangeBins bin{(float)weight.top, state.per};
+    const float from = best == INFINITY ? INFINITY : -3.402823466e38f;
+    Row<T, NT, IN_MEMORY, false> row;
+    row.open(logits + (int64_t)r * ld + first, min(chunk, V - first));
+    Mass mass{weight, best, from, ~0u, q.floor_z};
+    int b0 = 0;
+    u64 need = 0, sum = 0;
+    if (state.pending == 1) {
+        const u64* hist = split.hist(r);
+        need = find_bin<NT>(sm, [&](int b) { return hist[b]; }, [&](u64 of) { return q.prefix_mass(of); });
+        b0 = sm.bin;
+        need -= sm.above;
+        if (tid == 0) sm.count = 0;
+        __syncthreads();
+        row.each_pack([&](const auto& p, int at) {
+            constexpr int VEC = Elem<T>::VEC;
+            u64 a[VEC];
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) a[j] = weight(Elem<T>::value(p.e[j]));
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                const float x = Elem<T>::value(p.e[j]);
+                const int b = bin(x);
+                const bool low = (x != best) & ((double)x - (double)best < q.floor_z);
+                sum += x >= from && b < b0 && !low ? a[j] : 0;
+                if (x >= from && b == b0) {
+                    const int to = atomicAdd(&sm.count, 1);
+                    if (to < ROOM) sm.hist[to] = composite(order_key(x), first + at + j);
+                }
+            }
+        });
+    } else {
+        row.each_pack([&](const auto& p, int at) {
+#pragma unroll
+            for (int j = 0; j < Elem<T>::VEC; ++j) sum += mass(Elem<T>::value(p.e[j]), at + j);
+        });
+    }
+    sum = wave_sum_u64(sum);
+    if (lane == 0) __hip_atomic_store(&split.pieces(r)[blockIdx.x * WAVES + wave], sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    if (state.pending == 1) {   // this chunk's entries of the range, behind those of the chunks before
+        const int n = sm.count;
+        if (tid == 0) sm.index = (int)atomicAdd(&split.state(r)->listed, (unsigned)n);
+        __syncthreads();
+        const int to = sm.index + tid;
+        if (tid < min(n, ROOM) && to < ROOM)
+            __hip_atomic_store(&split.list(r)[to], sm.hist[tid], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    // The last workgroup to get here draws.  What it reads of the others they have stored at agent scope (past their XCD's
+    // cache), every wave has waited for its stores when one thread counts the workgroup in, and it is loaded at agent
+    // scope: no fence, which would write the XCD's whole cache back (64 rows of 131072 took 92 us in this launch with one
+    // in every wave).
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (tid == 0)
+        sm.flag = __hip_atomic_fetch_add(&split.state(r)->ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
+    __syncthreads();
+    if (!sm.flag) return;
+    const int count = (int)gridDim.x * WAVES;
+    for (int p = tid; p < count; p += NT) pieces[p] = __hip_atomic_load(&split.pieces(r)[p], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    // entries of a wave's piece of chunk c, as Row::open cuts it (the last chunk may be shorter than the others)
+    auto piece_of = [&](int c) {
+        constexpr int VEC = Elem<T>::VEC;
+        return (min(chunk, V - c * chunk) + NT * VEC - 1) / (NT * VEC) * 64 * VEC;
+    };
+    __syncthreads();
+    if (state.pending == 1) {
+        const int n = (int)__hip_atomic_load(&split.state(r)->listed, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (n > ROOM) {   // more equal values than that: the whole row on this workgroup
+            Row<T, NT, IN_MEMORY, false> long_row;
+            long_row.open(logits + (int64_t)r * ld, V);
+            u64 total = 0;
+            const u64 cut = find_cut<NT>(long_row, sm, true, (u64)(best == INFINITY ? kKeyPlusInf : kKeyFinite) << 32, weight,
+                                         q.span(V, S), [&](u64 of) { return q.prefix_mass(of); }, total);
+            const Mass kept{weight, best, value_of(cut), ~(unsigned)cut, q.floor_z};
+            total = wave_totals<NT>(long_row, sm, kept);
+            const int token = locate<NT>(long_row, sm, q.target(total), kept);
+            if (tid == 0) q.write(out, r, token, long_row.entry(token), best, total, S);
+            return;
+        }
+        if (tid < n) sm.hist[tid] = __hip_atomic_load(&split.list(r)[tid], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __syncthreads();
+        const u64 c = ranked<NT>(n, sm);
+        const float x = value_of(c);
+        const u64 w = c ? weight(x) : 0;
+        const u64 before = block_prefix<NT>(w, sm);
+        if (c && before < need) {
+            const int i = index_of(c);
+            if (before + w >= need) sm.cut = c;
+            if (!((x != best) & ((double)x - (double)best < q.floor_z))) atomicAdd(&pieces[i / chunk * WAVES + i % chunk / piece_of(i / chunk)], w);
+        }
+        __syncthreads();
+        mass.cut_x = value_of(sm.cut);
+        mass.cut_index = ~(unsigned)sm.cut;
+    }
+    const u64 mine = tid < count ? pieces[tid] : 0, before = block_prefix<NT>(mine, sm), total = sm.total, target = q.target(total);
+    if (target >= before && target - before < mine) {   // the piece that the draw falls into
+        sm.index = tid;
+        sm.above = target - before;
+    }
+    __syncthreads();
+    // within it: as locate() does, on a row of one wave that begins there
+    const int at = sm.index, c = at / WAVES, piece = piece_of(c), offset = at % WAVES * piece, begin = c * chunk + offset;
+    u64 left = sm.above;
+    if (wave == 0) {
+        Row<T, 64, IN_MEMORY, false> part;
+        part.open(logits + (int64_t)r * ld + begin, min(piece, min(chunk - offset, V - begin)));
+        bool found = false;
+        for (int i = 0; i < part.vectors && !found; ++i) {
+            const auto p = part.fetch(i);
+            const int at0 = begin + part.first + i * 64 * part.VEC;
+            u64 own = 0;
+            part.vector(p, at0, [&](float y, int e) { own += mass(y, e); });
+            u64 inc = own;
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const u64 up = __shfl_up(inc, o, 64);
+                if (lane >= o) inc += up;
+            }
+            const u64 sum_all = __shfl(inc, 63, 64);
+            if (left >= sum_all) {
+                left -= sum_all;
+                continue;
+            }
+            found = true;
+            if (left >= inc - own && left < inc) {
+                u64 run = inc - own;
+                bool done = false;
+                part.vector(p, at0, [&](float y, int e) {
+                    run += mass(y, e);
+                    if (!done && run > left) { q.write(out, r, e, y, best, total, S); done = true; }
+                });
+            }
+        }
+    }
 }
 
 // ---------------------------------------------------------------------------------------------- top-k and log-normaliser
@@ -727,12 +985,34 @@ constexpr int MAX_K = 1024, MAX_V = 1 << 22;
     } while (0)
 }  // namespace
 
+namespace {
+// Entries per workgroup where rows are split (a multiple of what its threads read at once), or 0: not split.  About 512
+// workgroups, two a CU; 32 bit, top-p 0.9, one workgroup a row against split (us a call):
+//   V        1 row          16             64             128
+//   32768    38.6 / 21.8    41.4 / 23.4    42.8 / 30.1    45.8 / 38.6
+//   50257    56.6 / 22.4    59.6 / 25.2    59.5 / 38.2    63.0 / 56.0
+//   131072    116 / 27.9     126 / 36.2     130 / 65.5     142 / 97.7
+// Shorter rows and more of them gain nothing.  Settings per row that leave no row to split cost 4 us (64 rows of 50257,
+// top-k 50: 15.5 against 19.3).
+int chunk_entries(int N, int V) {
+    if (V < 32768 || N > 128) return 0;
+    const int unit = CHUNK_NT * 8;
+    const int chunks = std::min(MAX_PIECES / (CHUNK_NT / 64), std::max(2, 512 / N));
+    const int64_t per = ((int64_t)V + chunks - 1) / chunks;
+    return (int)((per + unit - 1) / unit * unit);
+}
+}  // namespace
+
+extern "C" int64_t icrl_sample_filtered_work_bytes(int N, int V) {
+    return N > 0 && V > 0 && chunk_entries(N, V) ? (int64_t)N * WORK_WORDS * 8 : 0;
+}
+
 extern "C" int icrl_sample_tokens_filtered(const void* logits, int dtype, int64_t ld_logits, int N, int V,
                                            const double* uniforms, const float* temperature_rows, double temperature,
                                            const int32_t* top_k_rows, int top_k, const float* top_p_rows, double top_p,
                                            const float* min_p_rows, double min_p, int64_t* tokens_out,
-                                           int64_t token_stride, float* log_prob, int64_t log_prob_stride,
-                                           icrl_stream_t stream) {
+                                           int64_t token_stride, float* log_prob, int64_t log_prob_stride, void* work,
+                                           int64_t work_bytes, icrl_stream_t stream) {
     ICRL_REQUIRE(logits && uniforms && tokens_out && N > 0 && V > 0, "icrl_sample_tokens_filtered: null pointer or empty shape");
     ICRL_REQUIRE(ld_logits >= V, "icrl_sample_tokens_filtered: ld_logits < V");
     ICRL_REQUIRE(V <= MAX_V, "icrl_sample_tokens_filtered: vocabulary %d exceeds %d entries", V, MAX_V);
@@ -740,20 +1020,34 @@ extern "C" int icrl_sample_tokens_filtered(const void* logits, int dtype, int64_
     ICRL_REQUIRE(top_k_rows || top_k >= 0, "icrl_sample_tokens_filtered: top_k must not be negative (0: off)");
     ICRL_REQUIRE(top_p_rows || (top_p >= 0.0 && top_p <= 1.0), "icrl_sample_tokens_filtered: top_p must be in [0, 1]");
     ICRL_REQUIRE(min_p_rows || (min_p >= 0.0 && min_p <= 1.0), "icrl_sample_tokens_filtered: min_p must be in [0, 1]");
+    ICRL_REQUIRE(!work || (reinterpret_cast<uintptr_t>(work) % 8 == 0 && work_bytes >= icrl_sample_filtered_work_bytes(N, V)),
+                 "icrl_sample_tokens_filtered: work must be 8-byte aligned and hold icrl_sample_filtered_work_bytes(N, V) bytes");
     int bits = 0;
     while ((1 << bits) < V) ++bits;
     const int S = std::min(51, 62 - bits);
-    const Setting t{temperature_rows, temperature}, p{top_p_rows, top_p}, q{min_p_rows, min_p};
-#define ICRL_CALL(T, NT)                                                                                               \
-    hipLaunchKernelGGL((sample_filtered_kernel<T, NT>), dim3(N), dim3(NT), 0, icrl::as_stream(stream),                 \
-                       static_cast<const T*>(logits), ld_logits, V, S, uniforms, t, top_k_rows, top_k, p, q, tokens_out, \
-                       token_stride, log_prob, log_prob_stride)
+    const Requests all{uniforms, {temperature_rows, temperature}, {top_p_rows, top_p}, {min_p_rows, min_p}, top_k_rows, top_k};
+    const Results out{tokens_out, token_stride, log_prob, log_prob_stride};
+    // settings given once for all rows may say that a list settles every row: no launches for what would be left
+    const bool lists = (!top_k_rows && top_k > 0 && top_k < V) || (!temperature_rows && temperature == 0.0) ||
+                       (!top_p_rows && top_p == 1.0 && !min_p_rows && min_p > 0.0);
+    const int chunk = work && !lists ? chunk_entries(N, V) : 0;
+    const Work split{chunk ? static_cast<u64*>(work) : nullptr};
+    hipStream_t st = icrl::as_stream(stream);
+#define ICRL_CALL(T, NT) \
+    hipLaunchKernelGGL((sample_filtered_kernel<T, NT>), dim3(N), dim3(NT), 0, st, static_cast<const T*>(logits), ld_logits, V, S, all, out, split)
     // Two workgroups of 512 share a CU, one of 1024 has it to itself: wide ones pay where rows are long and there is a
-    // CU for each of them (64 rows of 131072: 122 against XX us; 333 of 50257: 57 against YY).
-#define ICRL_WIDTHS(T)                                          \
-    if (V <= 4096) { ICRL_CALL(T, 256); }                       \
-    else if (V <= 16384 || N > 256) { ICRL_CALL(T, 512); }      \
-    else { ICRL_CALL(T, 1024); }
+    // CU for each of them, with more rows than CUs the narrow ones (333 rows of 50257, min-p 0.05: 34 against 56 us).
+#define ICRL_WIDTHS(T)                                                                                                       \
+    if (V <= 4096) { ICRL_CALL(T, 256); }                                                                                    \
+    else if (V <= 16384 || N > 256) { ICRL_CALL(T, 512); }                                                                   \
+    else { ICRL_CALL(T, 1024); }                                                                                             \
+    if (chunk) {                                                                                                            \
+        const dim3 grid((V + chunk - 1) / chunk, N);                                                                         \
+        hipLaunchKernelGGL(sample_chunk_mass<T>, grid, dim3(CHUNK_NT), 0, st, static_cast<const T*>(logits), ld_logits, V, chunk, S, \
+                           all, split);                                                                                      \
+        hipLaunchKernelGGL(sample_chunk_draw<T>, grid, dim3(CHUNK_NT), 0, st, static_cast<const T*>(logits), ld_logits, V, chunk, S, \
+                           all, out, split);                                                                                 \
+    }
     switch (dtype) {
         case ICRL_F32: ICRL_WIDTHS(float); break;
         case ICRL_BF16: ICRL_WIDTHS(__bf16); break;

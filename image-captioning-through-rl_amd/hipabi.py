@@ -97,7 +97,8 @@ SIGNATURES = {
                                              c_vp, c_i64, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp]),
     "icrl_policy_rollout_rounds": (c_int, [c_vp] * 6 + [c_i64] + [c_int] * 5 + [c_vp] * 10),
     "icrl_sample_tokens_filtered": (c_int, [c_vp, c_int, c_i64, c_int, c_int, c_vp, c_vp, c_f64, c_vp, c_int, c_vp, c_f64,
-                                            c_vp, c_f64, c_vp, c_i64, c_vp, c_i64, c_vp]),
+                                            c_vp, c_f64, c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_vp]),
+    "icrl_sample_filtered_work_bytes": (c_i64, [c_int, c_int]),
     "icrl_topk_lse_rows": (c_int, [c_vp, c_int, c_i64, c_int, c_int, c_int, c_f64, c_vp, c_vp, c_vp, c_vp]),
     "icrl_distill_loss": (c_int, [c_vp, c_int, c_i64, c_int, c_int, c_vp, c_vp, c_int, c_vp, c_f64, c_vp, c_vp, c_vp, c_vp,
                                   c_i64, c_vp]),
@@ -594,11 +595,19 @@ def sample_tokens_filtered(logits, tokens_out, token_stride, uniforms, *, temper
         if isinstance(all_[i], torch.Tensor):
             _on_current_device(logits, all_[i])
             rows[i], all_[i] = _vector(all_[i], n, dtype, name), 0
+    need, work = load().icrl_sample_filtered_work_bytes(n, v), None
+    if need:   # few long rows: a place for the workgroups that share a row, in the order of the stream that they run on
+        if STREAM is None:
+            work = torch.empty(need, dtype=torch.uint8, device=logits.device)
+        else:
+            with torch.cuda.stream(_torch_stream()):
+                work = torch.empty(need, dtype=torch.uint8, device=logits.device)
     _check(load().icrl_sample_tokens_filtered(logits.data_ptr(), _dtype_code(logits), _row_stride(logits), n, v,
                                               _vector(uniforms, n, torch.float64, "uniforms"), rows[0], all_[0], rows[1],
                                               min(int(all_[1]), v), rows[2], all_[2], rows[3], all_[3],
                                               tokens_out.data_ptr(), token_stride,
-                                              None if log_prob is None else log_prob.data_ptr(), log_prob_stride, _stream()),
+                                              None if log_prob is None else log_prob.data_ptr(), log_prob_stride,
+                                              None if work is None else work.data_ptr(), need, _stream()),
            "icrl_sample_tokens_filtered")
 
 

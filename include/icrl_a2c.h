@@ -339,13 +339,16 @@ int icrl_topk_rows(const float* logits, int64_t ld_logits, int N, int V, int k, 
  * that holds a NaN or no entry above -inf, or whose settings are out of range (temperature negative or not finite,
  * top_k negative, top_p or min_p outside [0, 1], u NaN), draws nothing: token -1, log_prob NaN.
  * Weights are whole multiples of 2^-S of the largest (S = 62 - ceil(log2 V), at most 51), so sums are exact and the
- * result does not depend on how a row is split. */
+ * result does not depend on how a row is split.  work (optional): icrl_sample_filtered_work_bytes(N, V) bytes, 8-byte
+ * aligned, written anew by every call and free when it has run; few long rows are then split over workgroups (where that
+ * size is 0, or without it, each row has one). */
+int64_t icrl_sample_filtered_work_bytes(int N, int V);
 int icrl_sample_tokens_filtered(const void* logits, int dtype, int64_t ld_logits, int N, int V,
                                 const double* uniforms, const float* temperature_rows, double temperature,
                                 const int32_t* top_k_rows, int top_k, const float* top_p_rows, double top_p,
                                 const float* min_p_rows, double min_p, int64_t* tokens_out,
                                 int64_t token_stride, float* log_prob, int64_t log_prob_stride,
-                                icrl_stream_t stream);
+                                void* work, int64_t work_bytes, icrl_stream_t stream);
 
 /* icrl_topk_rows for any of the three dtypes, V <= 4194304 and k <= 1024, with the row's log-normaliser: values
  * [N, k] and indices [N, k] of the k largest entries in descending order, ties by lowest index (NaN after -inf);

@@ -571,3 +571,82 @@ def test_sampling_lists_of_every_length(kept):
         for s in (dict(min_p=0.1), dict(min_p=0.1, top_p=0.8), dict(top_k=kept), dict(top_k=kept, top_p=0.5, min_p=0.2)):
             tokens, lp = draw(x, u, **s)
             check_draw(x, u, s, tokens, lp)
+
+
+# rows that several workgroups share (few and long ones) and rows that one has to itself
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,v", [(1, 32768), (1, 262143), (2, 40961), (16, 131072), (33, 50257), (128, 32771)])
+def test_sampling_shared_rows_are_those_of_one_workgroup(n, v, dtype):
+    x = rows_of(n, v, dtype, n + v, pad=1, offset=1)
+    many = x.repeat(129 // n + 1, 1)[:129 + n]   # more rows: one workgroup each
+    assert hip.load().icrl_sample_filtered_work_bytes(n, v) > 0
+    assert hip.load().icrl_sample_filtered_work_bytes(many.shape[0], v) == 0
+    rs = np.random.RandomState(v)
+    for s in (dict(), dict(top_p=0.9), dict(top_p=0.4, temperature=2.0), dict(top_p=0.97, min_p=1e-4), dict(min_p=1e-7),
+              dict(top_p=0.9999999), dict(top_p=1e-9, temperature=0.7)):
+        u = rs.random_sample(n)
+        u[0] = 0.0 if "min_p" in s else 1.0 - 2.0 ** -53
+        tokens, lp = draw(x, u, **s)
+        check_draw(x[:2], u[:2], s, tokens[:2], lp[:2])
+        one, one_lp = draw(many, np.tile(u, 129 // n + 2)[:many.shape[0]], **s)
+        np.testing.assert_array_equal(tokens, one[:n])
+        np.testing.assert_array_equal(lp, one_lp[:n])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_sampling_shared_rows_with_ties_masks_and_settings_of_their_own(dtype):
+    n, v = 12, 50257
+    x = rows_of(n, v, dtype, 31)
+    x[0] = 1.0                                # one value throughout: the range of the cut holds the whole row
+    x[1] = -INF                               # nothing left
+    x[2, :] = -INF
+    x[2, 50256] = 3.0                         # the last word alone
+    x[3, 11], x[3, 50000] = INF, INF
+    x[4, 7000] = NAN
+    x[5, 4096:] = -INF                        # the first workgroup's words alone
+    x[6, ::2] = torch.finfo(dtype).min
+    x[7, 20000:20600] = 2.0                   # more equal words than the list of the range holds
+    x[7, :20000] = -9.0
+    x[7, 20600:] = -9.0
+    s = dict(temperature=torch.tensor([1.0] * 8 + [0.0, 0.8, 1.3, 1.0]).cuda(),
+             top_k=torch.tensor([0] * 8 + [0, 30, 0, 2000], dtype=torch.int32).cuda(),
+             top_p=torch.tensor([0.5, 0.9, 0.9, 0.9, 0.9, 0.7, 0.8, 0.3, 0.9, 0.9, 1.0, 0.9]).cuda(),
+             min_p=torch.tensor([0.0] * 10 + [0.25, 0.0]).cuda())
+    u = np.random.RandomState(8).random_sample(n)
+    want_work = hip.load().icrl_sample_filtered_work_bytes(n, v)
+    assert want_work > 0
+    for _ in range(2):   # what one call leaves in its place does not reach the next
+        tokens, lp = draw(x, u, **s)
+        check_draw(x, u, s, tokens, lp)
+
+
+def test_sampling_shared_rows_captured_twice():
+    """Two captured graphs and eager calls, each with a place of its own for the workgroups that share a row."""
+    n, v = 4, 60000
+    xs = [rows_of(n, v, F32, 40 + i) for i in range(2)]
+    u = torch.rand(n, dtype=torch.float64, generator=torch.Generator().manual_seed(6)).cuda()
+    tokens = [torch.empty(n, dtype=torch.int64, device="cuda") for _ in range(3)]
+
+    def call(x, out):
+        hip.sample_tokens_filtered(x, out, 1, u, top_p=0.9)
+
+    for i in range(2):
+        call(xs[i], tokens[i])
+    torch.cuda.synchronize()
+    graphs, side = [torch.cuda.CUDAGraph() for _ in range(2)], torch.cuda.Stream()
+    for i in range(2):
+        with torch.cuda.graph(graphs[i], stream=side):
+            call(xs[i], tokens[i])
+    for step in range(4):
+        for x in xs:
+            x.normal_(generator=torch.Generator(device="cuda").manual_seed(step)).mul_(2.0)
+        u.uniform_(generator=torch.Generator(device="cuda").manual_seed(step))
+        torch.cuda.synchronize()
+        graphs[0].replay()
+        with torch.cuda.stream(side):
+            graphs[1].replay()
+        torch.cuda.synchronize()
+        for i in range(2):
+            call(xs[i], tokens[2])
+            torch.cuda.synchronize()
+            assert torch.equal(tokens[i], tokens[2]), (step, i)

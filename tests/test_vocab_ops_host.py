@@ -20,7 +20,7 @@ def refused(name, *args, match):
 
 
 SAMPLE = dict(logits=A, dtype=0, ld=100, n=4, v=100, u=A, t_rows=None, t=1.0, k_rows=None, k=0, p_rows=None, p=1.0,
-              m_rows=None, m=0.0, out=A, stride=1, lp=None, lps=1, stream=None)
+              m_rows=None, m=0.0, out=A, stride=1, lp=None, lps=1, work=None, nwork=0, stream=None)
 
 
 @pytest.mark.parametrize("change,match", [
@@ -28,7 +28,8 @@ SAMPLE = dict(logits=A, dtype=0, ld=100, n=4, v=100, u=A, t_rows=None, t=1.0, k_
     (dict(n=0), "empty shape"), (dict(v=0), "empty shape"), (dict(ld=99), "ld_logits < V"), (dict(dtype=7), "dtype"),
     (dict(v=(1 << 22) + 1, ld=1 << 23), "exceeds"), (dict(t=-1.0), "temperature"), (dict(t=float("nan")), "temperature"),
     (dict(t=float("inf")), "temperature"), (dict(k=-1), "top_k"), (dict(p=-0.1), "top_p"), (dict(p=1.5), "top_p"),
-    (dict(p=float("nan")), "top_p"), (dict(m=1.01), "min_p"), (dict(m=float("nan")), "min_p")])
+    (dict(p=float("nan")), "top_p"), (dict(m=1.01), "min_p"), (dict(m=float("nan")), "min_p"),
+    (dict(v=100000, ld=100000, work=A, nwork=1000), "work"), (dict(work=A + 4), "work")])
 def test_sample_filtered_refuses(change, match):
     refused("icrl_sample_tokens_filtered", *dict(SAMPLE, **change).values(), match=match)
 
