@@ -53,7 +53,7 @@ struct alignas(16) Out { T e[VEC]; };
 template <typename T, int NT, int NV, typename F>
 __device__ __forceinline__ void write_row(const Row<T, NT, NV, false>& row, T* dst, F&& f) {
     constexpr int VEC = Elem<T>::VEC;
-    row.each_pack([&](const typename Row<T, NT, NV, false>::Pack& p, int at) {
+    row.sweep([&](const typename Row<T, NT, NV, false>::Pack& p, int at) {
         Out<T, VEC> o;
 #pragma unroll
         for (int j = 0; j < VEC; ++j) o.e[j] = from_float<T>(f(Elem<T>::value(p.e[j])));
@@ -162,7 +162,7 @@ __global__ __launch_bounds__(NT, 4) void distill_kernel(const T* logits, int64_t
     };
     if constexpr (ONLINE) {
         __syncthreads();   // the bitmap is whole
-        row.each_pack([&](const auto& p, int at) {
+        row.sweep([&](const auto& p, int at) {
             float top = best;
 #pragma unroll
             for (int j = 0; j < Elem<T>::VEC; ++j) top = fmaxf(top, Elem<T>::value(p.e[j]));

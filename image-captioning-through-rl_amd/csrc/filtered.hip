@@ -427,7 +427,7 @@ __device__ __forceinline__ int collect(const R& row, Shared<NT>& sm, float bound
     __syncthreads();
     u64 mine[2] = {0, 0};
     int n = 0;
-    row.each_pack([&](const typename R::Pack& p, int at) {
+    row.sweep([&](const typename R::Pack& p, int at) {
         float most = -INFINITY;
 #pragma unroll
         for (int j = 0; j < R::VEC; ++j) most = fmaxf(most, Elem<typename R::Type>::value(p.e[j]));
@@ -569,10 +569,14 @@ __global__ __launch_bounds__(NT, 4) void sample_filtered_kernel(const T* __restr
         if (split.rows) split.state(r)->pending = 0;
     }
     float best = -INFINITY;
-    bool nan = false;
-    row.each([&](float x, int) {
-        best = fmaxf(best, x);                       // fmaxf passes over NaN
-        nan |= x != x;
+    u64 nan = 0;                                     // the wave's lanes
+    row.sweep([&](const auto& p, int) {
+#pragma unroll
+        for (int j = 0; j < Elem<T>::VEC; j += 2) {
+            const float x = Elem<T>::value(p.e[j]), y = Elem<T>::value(p.e[j + 1]);
+            best = fmaxf(best, fmaxf(x, y));         // fmaxf passes over NaN
+            nan |= __ballot(__builtin_isunordered(x, y));
+        }
     });
     const float own = best;
     best = block_max<NT>(best, sm.red);
@@ -590,7 +594,7 @@ __global__ __launch_bounds__(NT, 4) void sample_filtered_kernel(const T* __restr
         __syncthreads();
         if (own == best) {
             int first = V;
-            row.each([&](float x, int i) { first = x == best ? min(first, i) : first; });
+            row.sweep_each([&](float x, int i) { first = x == best ? min(first, i) : first; });
             atomicMin(&sm.index, first);
         }
         __syncthreads();
@@ -920,7 +924,7 @@ __global__ __launch_bounds__(NT, 8) void topk_lse_kernel(const T* __restrict__ l
     float best = -INFINITY;
     bool nan = false;
     if (tid == 0) sm.flag = 0;
-    row.each([&](float x, int) {
+    row.sweep_each([&](float x, int) {
         best = fmaxf(best, x);
         nan |= x != x;
     });
@@ -932,7 +936,7 @@ __global__ __launch_bounds__(NT, 8) void topk_lse_kernel(const T* __restrict__ l
         float part = 0.f;
         if (some) {
             const float c = (float)(per_t * 1.4426950408889634074);
-            row.each([&](float x, int) { part += __builtin_amdgcn_exp2f((x - best) * c); });
+            row.sweep_each([&](float x, int) { part += __builtin_amdgcn_exp2f((x - best) * c); });
         }
         double s = wave_sum_d((double)part);
         if ((tid & 63) == 0) sums[tid >> 6] = s;

@@ -57,22 +57,18 @@ struct Row {
 
     // Vector i, 16 bytes where the row has them.  Rows in memory: the one vector that the row ends inside of is read when
     // the row is opened, entry by entry, and handed out by the thread that owns it (nothing of that is left in the passes).
-    __device__ __forceinline__ Pack read(int i) const {
+    __device__ __forceinline__ Words read(int i) const {
         const int at = first + i * 64 * VEC;
         if constexpr (PLACE == IN_MEMORY) {
-            if (wave_first + (i + 1) * 64 * VEC <= V) return __builtin_bit_cast(Pack, *reinterpret_cast<const Words*>(src + at));
+            if (wave_first + (i + 1) * 64 * VEC <= V) return *reinterpret_cast<const Words*>(src + at);
             Words w = at < V ? __builtin_bit_cast(Words, end) : __builtin_bit_cast(Words, fill());
             if (at + VEC <= V) w = *reinterpret_cast<const Words*>(src + at);
-            return __builtin_bit_cast(Pack, w);
+            return w;
         } else {
-            Pack p;
-            if (at + VEC <= V) {
-                p = __builtin_bit_cast(Pack, *reinterpret_cast<const Words*>(src + at));
-            } else {
-                p = fill();
-                read_end(p, at);
-            }
-            return p;
+            if (at + VEC <= V) return *reinterpret_cast<const Words*>(src + at);
+            Pack p = fill();
+            read_end(p, at);
+            return __builtin_bit_cast(Words, p);
         }
     }
     __device__ __forceinline__ void read_end(Pack& p, int at) const {
@@ -86,7 +82,8 @@ struct Row {
         for (int j = 0; j < VEC; ++j) p.e[j] = kFill;
         return p;
     }
-    __device__ __forceinline__ Pack canonical(Pack p, int i) const {
+    __device__ __forceinline__ Pack canonical(Words w, int i) const {
+        Pack p = __builtin_bit_cast(Pack, w);
         const int at = first + i * 64 * VEC;
         if (CANON) {
 #pragma unroll
@@ -141,17 +138,57 @@ struct Row {
                 if (i < vectors) f(pass(keep[i]), first + i * 64 * VEC);
         } else {
             constexpr int AHEAD = 4;   // reads in flight: a queue in registers
-            Pack p[AHEAD];
+            Words p[AHEAD];            // (as words: packs of 16-bit entries are taken apart on arrival, which waits for them)
 #pragma unroll
             for (int q = 0; q < AHEAD; ++q)
                 if (q < vectors) p[q] = read(q);
 #pragma unroll 1
             for (int i = 0; i < vectors; ++i) {
-                const Pack now = p[0];
+                const Words now = p[0];
 #pragma unroll
                 for (int q = 0; q + 1 < AHEAD; ++q) p[q] = p[q + 1];
                 if (i + AHEAD < vectors) p[AHEAD - 1] = read(i + AHEAD);
                 f(canonical(now, i), first + i * 64 * VEC);
+            }
+        }
+    }
+    // The same for an f of few instructions, which leaves a pass waiting for its reads: four vectors are always on their
+    // way, at the price of f's code five times.  (The queue above moves what it has just asked for and so waits for it one
+    // vector later; gradient of 512 x 131072 bf16 50.4 against 45.7 us.)  Places past the end are handed out in the row's
+    // last vector only.
+    template <typename F>
+    __device__ __forceinline__ void sweep(F&& f) const {
+        if constexpr (PLACE > 0) {
+            each_pack(f);
+        } else {
+            constexpr int AHEAD = 4, STEP = 64 * VEC;
+            const int left = V - wave_first, live = min(vectors, left > 0 ? (left + STEP - 1) / STEP : 0);
+            const int whole = left > 0 ? min(vectors, left / STEP) : 0;
+            int i = 0;
+            if (whole >= AHEAD) {
+                Words p[AHEAD];
+#pragma unroll
+                for (int q = 0; q < AHEAD; ++q) p[q] = *reinterpret_cast<const Words*>(src + first + q * STEP);
+#pragma unroll 1
+                for (; i + AHEAD <= whole; i += AHEAD) {
+#pragma unroll
+                    for (int q = 0; q < AHEAD; ++q) {
+                        const Words now = p[q];
+                        p[q] = *reinterpret_cast<const Words*>(src + first + min(i + AHEAD + q, whole - 1) * STEP);
+                        f(canonical(now, i + q), first + (i + q) * STEP);
+                    }
+                }
+            }
+            Words p[AHEAD];   // at most three whole ones and the last
+#pragma unroll
+            for (int q = 0; q < AHEAD; ++q)
+                if (i + q < live) p[q] = read(i + q);
+#pragma unroll 1
+            for (; i < live; ++i) {
+                const Words now = p[0];
+#pragma unroll
+                for (int q = 0; q + 1 < AHEAD; ++q) p[q] = p[q + 1];
+                f(canonical(now, i), first + i * STEP);
             }
         }
     }
@@ -164,6 +201,10 @@ struct Row {
     template <typename F>
     __device__ __forceinline__ void each(F&& f) const {
         each_pack([&](const Pack& p, int at) { vector(p, at, f); });
+    }
+    template <typename F>
+    __device__ __forceinline__ void sweep_each(F&& f) const {
+        sweep([&](const Pack& p, int at) { vector(p, at, f); });
     }
 };
 
