@@ -314,6 +314,20 @@ int check(const char* who, const void* logits, int64_t ld, int N, int V, const v
     ICRL_REQUIRE(temperature > 0.0 && isfinite(temperature), "%s: temperature must be positive and finite", who);
     return ICRL_OK;
 }
+
+// The gradient's rows are the logits' own places, or share none with them: a row may be written while others are read.
+bool same_or_apart(const void* logits, int64_t ld, const void* dlogits, int64_t ldd, int N, int V, int64_t size) {
+    const intptr_t a = reinterpret_cast<intptr_t>(logits), b = reinterpret_cast<intptr_t>(dlogits);
+    if (a == b && (ld == ldd || N == 1)) return true;
+    if (a + ((N - 1) * ld + V) * size <= b || b + ((N - 1) * ldd + V) * size <= a) return true;
+    if (ld != ldd || N == 1) return false;
+    const int64_t row = ld * size, shift = (((b - a) % row) + row) % row;   // side by side in the rows of one matrix
+    return shift >= V * size && row - shift >= V * size;
+}
+#define ICRL_REQUIRE_PLACES(who)                                                                                    \
+    ICRL_REQUIRE(!dlogits || dtype < ICRL_F32 || dtype > ICRL_F16 ||                                                \
+                     same_or_apart(logits, ld_logits, dlogits, ld_dlogits, N, V, dtype == ICRL_F32 ? 4 : 2),        \
+                 who ": dlogits overlaps the logits without being them")
 }  // namespace
 
 extern "C" int icrl_distill_loss(const void* logits, int dtype, int64_t ld_logits, int N, int V, const float* teacher_values,
@@ -324,6 +338,7 @@ extern "C" int icrl_distill_loss(const void* logits, int dtype, int64_t ld_logit
     ICRL_REQUIRE(row_loss, "icrl_distill_loss: null pointer or empty shape");
     ICRL_REQUIRE(reinterpret_cast<uintptr_t>(stats) % 8 == 0, "icrl_distill_loss: stats must be 8-byte aligned");
     ICRL_REQUIRE(!dlogits || ld_dlogits >= V, "icrl_distill_loss: ld_dlogits < V");
+    ICRL_REQUIRE_PLACES("icrl_distill_loss");
     const size_t lds = (size_t)((V + 31) / 32) * 4;
 #define ICRL_CALL(T, NT, NV)                                                                                            \
     hipLaunchKernelGGL((distill_kernel<T, NT, NV>), dim3(N), dim3(NT), lds, icrl::as_stream(stream),                    \
@@ -347,6 +362,7 @@ extern "C" int icrl_distill_grad(const void* logits, int dtype, int64_t ld_logit
     ICRL_REQUIRE(stats && dlogits, "icrl_distill_grad: null pointer or empty shape");
     ICRL_REQUIRE(reinterpret_cast<uintptr_t>(stats) % 8 == 0, "icrl_distill_grad: stats must be 8-byte aligned");
     ICRL_REQUIRE(ld_dlogits >= V, "icrl_distill_grad: ld_dlogits < V");
+    ICRL_REQUIRE_PLACES("icrl_distill_grad");
 #define ICRL_CALL(T, NT, NV)                                                                                           \
     hipLaunchKernelGGL((distill_grad_kernel<T, NT, NV>), dim3(N), dim3(NT), 0, icrl::as_stream(stream),                \
                        static_cast<const T*>(logits), ld_logits, V, teacher_values, teacher_indices, k,                \

@@ -640,7 +640,6 @@ def _distill_operands(logits, teacher_values, teacher_indices, dlogits, stats):
     assert teacher_indices.is_contiguous()
     if dlogits is not None:
         assert dlogits.shape == logits.shape and dlogits.dtype == logits.dtype, "dlogits must be shaped and typed like the logits"
-        assert dlogits.data_ptr() != logits.data_ptr() or _row_stride(dlogits) == _row_stride(logits)
     assert stats is None or (stats.dtype == torch.float64 and stats.is_contiguous() and stats.numel() == 4 * n), \
         "stats must be %d contiguous float64" % (4 * n)
     return n, k

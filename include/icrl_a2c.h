@@ -364,7 +364,7 @@ int icrl_topk_lse_rows(const void* logits, int dtype, int64_t ld_logits, int N, 
  *     word with q_r = max(0, 1 - sum q_j) and p_r = their p together (left out where the policy has no mass there);
  *   teacher_lse null: q = softmax(value / temperature) over the list.
  *   row_loss = row_weight * (sum_j q_j log(q_j / p_j) + q_r log(q_r / p_r));
- *   dlogits (optional; same dtype as logits, which it may be itself) = its gradient.
+ *   dlogits (optional; same dtype as logits, which it may be itself, but no other overlap) = its gradient.
  * teacher_values / teacher_indices: [N, k], k <= 1024, V <= 262144; a negative index is an absent entry (its value is
  * not read), an index >= V or one that occurs twice in a row makes that row's results NaN; a row without entries has
  * loss and gradient 0.  row_weight (optional) [N]; rows of weight 0 are not read, their results are zeros.  stats

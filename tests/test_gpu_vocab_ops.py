@@ -650,3 +650,18 @@ def test_sampling_shared_rows_captured_twice():
             call(xs[i], tokens[2])
             torch.cuda.synchronize()
             assert torch.equal(tokens[i], tokens[2]), (step, i)
+
+
+def test_distillation_gradient_beside_the_logits_in_one_matrix():
+    n, v = 6, 1000
+    both = torch.empty(n, 2 * v + 3, device="cuda")
+    x = rows_of(n, v, F32, 50)
+    both[:, :v] = x
+    both[:, v + 3:] = 7.0
+    tv, ti, lse = teacher_for(x, 9, 1.0, 51)
+    loss, one, apart = torch.empty(n, device="cuda"), torch.empty(n, device="cuda"), torch.empty(n, v, device="cuda")
+    hip.distill_loss(both[:, :v], tv, ti, loss, teacher_lse=lse, dlogits=both[:, v + 3:])
+    hip.distill_loss(x, tv, ti, one, teacher_lse=lse, dlogits=apart)
+    assert torch.equal(loss, one) and torch.equal(both[:, v + 3:], apart) and torch.equal(both[:, :v], x)
+    with pytest.raises(RuntimeError, match="overlaps"):
+        hip.distill_loss(both[:, :v], tv, ti, loss, teacher_lse=lse, dlogits=both[:, v - 1:2 * v - 1])

@@ -65,6 +65,14 @@ def test_distill_grad_refuses(change, match):
     refused("icrl_distill_grad", *dict(GRAD, **change).values(), match=match)
 
 
+# bf16, four rows of 100: one entry further, a row further, other strides from the same place, halves that overlap
+@pytest.mark.parametrize("ld,d,ldd", [(100, A + 2, 100), (100, A - 2, 100), (100, A + 200, 100), (100, A, 128), (150, A + 120, 150),
+                                      (250, A + 302, 250), (120, A + 120 * 2 * 3 + 198, 200)])
+def test_distill_refuses_gradients_that_overlap_the_logits(ld, d, ldd):
+    refused("icrl_distill_loss", *dict(LOSS, ld=ld, d=d, ldd=ldd).values(), match="overlaps")
+    refused("icrl_distill_grad", *dict(GRAD, ld=ld, d=d, ldd=ldd).values(), match="overlaps")
+
+
 CUT = dict(x=A, dtype=0, ld=64, rows=4, k=64, pieces=A, scales=A, stream=None)
 GEMM = dict(ap=A, as_=A, bp=A, bs=A, c=A, dtype=0, ldc=100, m=4, n=100, k=64, bias=None, stream=None)
 
