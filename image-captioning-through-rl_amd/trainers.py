@@ -409,11 +409,12 @@ def train_policy_network(train_data, network_paths, plot_dir, bidirectional, epo
 @torch.no_grad()
 def teacher_record(policy_network, features, captions, top=64, temperature=1.0):
     """What a trained policy network leaves for a student: for every teacher-forced position of captions [N, L] its `top`
-    largest logits (values, word indices: [(L - 1) N, top], position by position) and the log-normaliser of the whole
-    row at `temperature` [(L - 1) N]."""
+    largest logits (all of them if the vocabulary is smaller; values, word indices: [(L - 1) N, top], position by
+    position) and the log-normaliser of the whole row at `temperature` [(L - 1) N]."""
     caps = torch.as_tensor(np.asarray(captions) if not torch.is_tensor(captions) else captions)
     logits = policy_network(torch.as_tensor(features).unsqueeze(0), caps[:, :-1])       # [N, L - 1, V], stored [L - 1, N, V]
     rows = logits.permute(1, 0, 2).reshape(-1, logits.shape[2])
+    top = min(top, rows.shape[1])
     values = torch.empty(rows.shape[0], top, device=rows.device)
     indices = torch.empty(rows.shape[0], top, dtype=torch.int64, device=rows.device)
     lse = torch.empty(rows.shape[0], device=rows.device)

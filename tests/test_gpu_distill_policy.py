@@ -162,3 +162,16 @@ def test_decoding_with_the_eight_bit_vocabulary_matrix(n):
     off = ((2.0 ** -3 + 2.0 ** -8) * w.sum(1) + 512 * 2.0 ** -10 / 224 * (w.max(1).values + 1.0) + 1e-4).max()
     chosen = logits.gather(2, tokens[:, 1:].unsqueeze(2)).squeeze(2)
     assert (chosen >= logits.max(2).values - 2 * off).all()
+
+
+def test_a_teachers_record_of_a_small_vocabulary_holds_all_of_it():
+    net = policy(40, 32, 3)
+    feats = torch.randn(4, 32, generator=torch.Generator().manual_seed(9)).cuda()
+    caps = torch.randint(0, 40, (4, 6), generator=torch.Generator().manual_seed(10)).cuda()
+    values, indices, lse = trainers.teacher_record(net, feats, caps, 64, 1.5)
+    assert values.shape == indices.shape == (20, 40) and lse.shape == (20,)
+    assert torch.equal(indices.sort(dim=1).values, torch.arange(40, device="cuda").expand(20, 40))
+    # the values are exact copies; float64 on the CPU sums them, so that the record's float32 is off by its own rounding, and
+    # by the 40 float32 exponentials' (2^-22 of the sum at most, each one's argument and result together)
+    want = torch.logsumexp(values.double().cpu() / 1.5, dim=1)
+    assert (lse.double().cpu() - want).abs().max() <= 2.0 ** -22 + 2.0 ** -24 * float(want.abs().max())

@@ -665,3 +665,14 @@ def test_distillation_gradient_beside_the_logits_in_one_matrix():
     assert torch.equal(loss, one) and torch.equal(both[:, v + 3:], apart) and torch.equal(both[:, :v], x)
     with pytest.raises(RuntimeError, match="overlaps"):
         hip.distill_loss(both[:, :v], tv, ti, loss, teacher_lse=lse, dlogits=both[:, v - 1:2 * v - 1])
+
+
+def test_sampling_shared_rows_at_extreme_temperatures():
+    """All weights alike, and none but the largest entry's."""
+    n, v = 3, 40000
+    x = rows_of(n, v, F32, 60)
+    x[:, 39999] = 30.0
+    u = np.array([0.0, 0.5, 0.999])
+    for s in (dict(temperature=1e30), dict(temperature=1e30, top_p=0.5), dict(temperature=1e-30), dict(temperature=1e-30, top_p=0.5)):
+        tokens, lp = draw(x, u, **s)
+        check_draw(x, u, s, tokens, lp)
