@@ -990,19 +990,20 @@ constexpr int MAX_K = 1024, MAX_V = 1 << 22;
 }  // namespace
 
 namespace {
-// Entries per workgroup where rows are split (a multiple of what its threads read at once), or 0: not split.  About 512
-// workgroups, two a CU; 32 bit, top-p 0.9, one workgroup a row against split (us a call):
+// Entries per workgroup where rows are split (a multiple of what its threads read at once), or 0: not split.  Where two
+// workgroups a CU are reached they get at least 8192 entries, up to four a CU, since rows that a list has settled leave
+// theirs idle.  32 bit, top-p 0.9, one workgroup a row against split (us a call):
 //   V        1 row          16             64             128
-//   32768    38.6 / 21.8    41.4 / 23.4    42.8 / 30.1    45.8 / 38.6
-//   50257    56.6 / 22.4    59.6 / 25.2    59.5 / 38.2    63.0 / 56.0
-//   131072    116 / 27.9     126 / 36.2     130 / 65.5     142 / 97.7
+//   32768    37.5 / 21.9    41.9 / 23.4    42.6 / 30.1    45.7 / 38.6
+//   50257    56.6 / 21.7    59.0 / 25.1    60.3 / 38.2    62.5 / 56.0
+//   131072    126 / 26.6     126 / 35.1     130 / 64.9     138 / 97.0
 // Shorter rows and more of them gain nothing.  Settings per row that leave no row to split cost 4 us (64 rows of 50257,
-// top-k 50: 15.5 against 19.3).
+// top-k 50: 14.4 against 18.8).
 int chunk_entries(int N, int V) {
     if (V < 32768 || N > 128) return 0;
     const int unit = CHUNK_NT * 8;
-    const int chunks = std::min(MAX_PIECES / (CHUNK_NT / 64), std::max(2, 512 / N));
-    const int64_t per = ((int64_t)V + chunks - 1) / chunks;
+    const int chunks = std::min(MAX_PIECES / (CHUNK_NT / 64), std::max(2, 1024 / N));
+    const int64_t even = ((int64_t)V + chunks - 1) / chunks, per = chunks * N > 512 ? std::max<int64_t>(even, 8192) : even;
     return (int)((per + unit - 1) / unit * unit);
 }
 }  // namespace
