@@ -7,8 +7,11 @@
 // Without the teacher's log-normaliser q is the softmax over the list and q_r = 0.
 //
 // Bound by memory: the forward pass reads the row once, the gradient writes it once; rows up to 32768 (65536) entries
-// of 4 (2) bytes stay in registers in between, longer ones are read again.  p_r is summed directly over the words outside (a bitmap of the list in LDS
-// tells them apart): as 1 - sum it would lose all its digits where the policy is sure.  Row sums are float32 per
+// of 4 (2) bytes stay in registers in between, longer ones are read again.  Measured: loss and gradient of 9728 x 10000
+// float32, k = 64, a fifth of the rows idle: 176 us for 700 MB, 4.0 TB/s (a plain copy reaches 4.8); 512 x 131072 bf16,
+// k = 128, in two calls, 5% idle: 103 us for 383 MB (the rows' sums take one CU each about as long as their reads).
+// p_r is summed directly over the words outside (a bitmap of the list in LDS tells them apart): as 1 - sum it would lose
+// all its digits where the policy is sure.  Row sums are float32 per
 // thread (at most a few hundred terms each) and float64 from there on; the handful of numbers per row and the list's
 // terms are float64 throughout, since the loss is a difference of nearly equal ones.
 #include <math.h>

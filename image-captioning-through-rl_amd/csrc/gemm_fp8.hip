@@ -30,6 +30,8 @@ constexpr int BLOCK = 128;
 inline int blocks128(int K) { return (K + BLOCK - 1) / BLOCK; }
 inline int scale_words(int K) { return (blocks128(K) + 3) / 4; }   // 32-bit words of scales per row
 
+// scale = the smallest power of two 2^e with max |x| <= 448 2^e over a row's block of 128, code = x / scale rounded once.
+// Bound by memory: 32000 x 2048 float32 98 us, 4096 x 2048 bf16 12-15 us; small operands by the launch (512 x 512: 2.6-4 us).
 // Eight lanes cut one row's block of 128: 16 entries a lane, which are one 16-byte half of the fragment's lane.
 template <typename T>
 __global__ __launch_bounds__(64) void cut_kernel(const T* __restrict__ x, int64_t ld, int rows, int K, int nblocks, int words,
@@ -136,6 +138,7 @@ template <typename T>
 using Fragment = std::conditional_t<sizeof(T) == 4, ExactFragment, ScaledFragment>;
 
 // ---- few rows: one 32 x 32 tile of the output per workgroup, k cut over its waves, fragments straight from memory
+// Bound by the launch and one trip to memory: 1 x 10000 x 512 takes 3.7 us for 5 MB.
 template <typename T, int WAVES>
 __global__ __launch_bounds__(WAVES * 64) void gemm_fp8_rows(Operand a, Operand b, T* __restrict__ out, int64_t ldo, int M, int N,
                                                             int nblocks, int words, const float* __restrict__ bias) {
@@ -174,6 +177,9 @@ __global__ __launch_bounds__(WAVES * 64) void gemm_fp8_rows(Operand a, Operand b
 // (of 1024 clocks of matrix instructions on 256 x 256 tiles) are in flight while one is multiplied, which covers the
 // latency of the caches behind the L2.  The fragments of the next stage are read from LDS into registers while the
 // current ones are multiplied, so one wave per SIMD keeps the matrix cores busy.
+// Measured: 4096 x 32000 x 2048 into bf16 324 us, 1650 TFLOP/s (a library product of 8192 cubed reaches 2740): the matrix
+// cores are busy 36% of the CUs' time, and a quarter of a wave's is spent in waits.  512 x 10000 x 512 into float32 13.5 us,
+// of which 20 MB of output take 3 and bf16's rate 4: workgroups of eight stages, bound by their beginnings and ends.
 template <typename T, int WM, int WN>
 __global__ __launch_bounds__(256) void gemm_fp8_tiles(Operand a, Operand b, T* __restrict__ out, int64_t ldo, int M, int N,
                                                       int nblocks, int words, const float* __restrict__ bias, int tiles_m,

@@ -7,6 +7,9 @@
 argument order and meaning, same logged scalar tags, same NumPy / torch RNG consumption (so the same
 seeds give the same minibatch order and the same sampled tokens as the reference).
 
+Without a counterpart there: ``GenerateCaptionsSampled`` (decoding under temperature, top-k, top-p and min-p) and
+``teacher_record`` / ``distill_policy_network`` (a policy network trained from another's top logits).
+
 With more than one process (torch.distributed initialised, one rank per GPU) every loop here is
 data-parallel: each rank takes its own rows of every global minibatch (utilities.sharded_minibatches),
 draws its sampling uniforms from its own NumPy stream, starts from rank 0's parameters, averages the
