@@ -182,6 +182,58 @@ __device__ __forceinline__ int locate(const R& row, Shared<NT>& sm, u64 target, 
     return sm.index;
 }
 
+// The same with the vectors of the piece summed side by side, one a wave, where f is long (512 rows of 10 000, top-p 0.9:
+// 33.3 against 31.7 us, 64 rows of 131072 without filters on a workgroup each 71 against 57; in the kernel that records rows
+// its registers would cost more: 44 against 55 us for 4096 x 10000).  sm.hist is free.
+template <int NT, typename R, typename F>
+__device__ __forceinline__ int locate_wide(const R& row, Shared<NT>& sm, u64 target, F&& f) {
+    constexpr int WAVES = NT / 64;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int piece = 0;
+    u64 left = target;
+#pragma unroll 1
+    while (piece < WAVES - 1 && left >= sm.part[piece]) left -= sm.part[piece++];
+    __syncthreads();   // (the histogram's last readers are done)
+#pragma unroll 1
+    for (int base = 0; base < row.vectors; base += WAVES) {
+        const int i = base + wave, at0 = ((piece * row.vectors + i) * 64 + lane) * R::VEC;
+        u64 own = 0;
+        typename R::Pack p = R::fill();
+        if (i < row.vectors) {
+            p = row.fetch_at(at0);
+            row.vector(p, at0, [&](float x, int at) { own += f(x, at); });
+        }
+        u64 inc = own;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const u64 up = __shfl_up(inc, o, 64);
+            if (lane >= o) inc += up;
+        }
+        if (lane == 63) sm.hist[wave] = inc;
+        __syncthreads();
+        u64 before = 0, all = 0;
+#pragma unroll 1
+        for (int w = 0; w < WAVES; ++w) {
+            const u64 s = sm.hist[w];
+            before += w < wave ? s : 0;
+            all += s;
+        }
+        if (left >= before + inc - own && left < before + inc) {   // one thread, if it is here at all
+            u64 run = before + inc - own;
+            bool done = false;
+            row.vector(p, at0, [&](float x, int at) {
+                run += f(x, at);
+                if (!done && run > left) { sm.index = at; done = true; }
+            });
+        }
+        if (left < all) break;
+        left -= all;
+        __syncthreads();
+    }
+    __syncthreads();
+    return sm.index;
+}
+
 // Where the running sum of the bins (bin_at(0) first) reaches `need` (which need_of makes from the total): bin in sm.bin, the
 // sum of the bins before it in sm.above.  Returns need.
 template <int NT, typename H, typename G>
@@ -555,8 +607,8 @@ struct Kept { u64 w; unsigned index, pad; };
 // of those w_i >= min_p; the token is the first kept one, by index, at which the running mass exceeds u times the total.
 // Bound by the arithmetic of the passes that weigh entries (about 45 instructions an entry, 20 of them float64; a top-p
 // over the whole row weighs it twice) and, with a list, by two reads of the row on one CU.  Measured (us a call): 1 row of
-// 10 000, top-k 50 and top-p 0.95: 10.4; 512 rows of 10 000, top-p 0.9: 33 (the rows' bytes alone take 5, the vector
-// instructions, 144 an entry altogether, 20); 333 rows of 50 257 f16, min-p 0.05: 31; 64 rows of 131 072 bf16, settings of their own, with the launches below: 54-61.
+// 10 000, top-k 50 and top-p 0.95: 10.4; 512 rows of 10 000, top-p 0.9: 31 (the rows' bytes alone take 5, the vector
+// instructions, 144 an entry altogether, 20); 333 rows of 50 257 f16, min-p 0.05: 31-34; 64 rows of 131 072 bf16, settings of their own, with the launches below: 54-61.
 // split.rows not null: rows that need the weights of all their entries are left to the launches that follow.
 template <typename T, int NT>
 __global__ __launch_bounds__(NT, 4) void sample_filtered_kernel(const T* __restrict__ logits, int64_t ld, int V, int S, Requests all,
@@ -722,12 +774,12 @@ __global__ __launch_bounds__(NT, 4) void sample_filtered_kernel(const T* __restr
     }
     const Mass mass{weight, best, value_of(cut), ~(unsigned)cut, floor_z};
     if (total == 0 || q.min_p > 0.0) total = wave_totals<NT>(row, sm, mass);
-    const int token = locate<NT>(row, sm, q.target(total), mass);
+    const int token = locate_wide<NT>(row, sm, q.target(total), mass);
     if (tid == 0) q.write(out, r, token, row.entry(token), best, total, S);
 }
 
 // ---- rows split over workgroups
-// A row's weights cost some 45 instructions an entry, twice (45 us a pass for 131072 entries on one CU), so where rows are
+// A row's weights cost some 45 instructions an entry, twice (40 us a pass for 131072 entries on one CU), so where rows are
 // long and few their chunks are weighed side by side: one launch adds the chunks' histograms up (integers: any order
 // gives the same), the next collects the range of the cut and the masses above it, and the workgroup that finishes last
 // with a row draws.  No workgroup waits for another.
@@ -856,7 +908,7 @@ __global__ __launch_bounds__(CHUNK_NT, 4) void sample_chunk_draw(const T* __rest
                                          q.span(V, S), [&](u64 of) { return q.prefix_mass(of); }, total);
             const Mass kept{weight, best, value_of(cut), ~(unsigned)cut, q.floor_z};
             total = wave_totals<NT>(long_row, sm, kept);
-            const int token = locate<NT>(long_row, sm, q.target(total), kept);
+            const int token = locate_wide<NT>(long_row, sm, q.target(total), kept);
             if (tid == 0) q.write(out, r, token, long_row.entry(token), best, total, S);
             return;
         }
@@ -1004,11 +1056,11 @@ namespace {
 // workgroups a CU are reached they get at least 8192 entries, up to four a CU, since rows that a list has settled leave
 // theirs idle.  32 bit, top-p 0.9, one workgroup a row against split (us a call):
 //   V        1 row          16             64             128
-//   32768    37.5 / 21.9    41.9 / 23.4    42.6 / 30.1    45.7 / 38.6
-//   50257    56.6 / 21.7    59.0 / 25.1    60.3 / 38.2    62.5 / 56.0
-//   131072    126 / 26.6     126 / 35.1     130 / 64.9     138 / 97.0
+//   32768    38.8 / 21.3    39.9 / 26.4    40.4 / 29.4    43.5 / 38.4
+//   50257    52.9 / 22.8    54.9 / 28.3    55.4 / 37.1    58.0 / 55.0
+//   131072    108 / 27.4     113 / 34.7     115 / 65.5     120 / 97.7
 // Shorter rows and more of them gain nothing.  Settings per row that leave no row to split cost 4 us (64 rows of 50257,
-// top-k 50: 14.4 against 18.8).
+// top-k 50: 14.6 against 18.8).
 int chunk_entries(int N, int V) {
     if (V < 32768 || N > 128) return 0;
     const int unit = CHUNK_NT * 8;

@@ -82,9 +82,9 @@ struct Row {
         for (int j = 0; j < VEC; ++j) p.e[j] = kFill;
         return p;
     }
-    __device__ __forceinline__ Pack canonical(Words w, int i) const {
+    __device__ __forceinline__ Pack canonical(Words w, int i) const { return canonical_at(w, first + i * 64 * VEC); }
+    __device__ __forceinline__ Pack canonical_at(Words w, int at) const {
         Pack p = __builtin_bit_cast(Pack, w);
-        const int at = first + i * 64 * VEC;
         if (CANON) {
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
@@ -96,6 +96,18 @@ struct Row {
     }
     __device__ __forceinline__ Pack fetch(int i) const {
         return canonical(read(i), i);
+    }
+    // the vector of any thread: 16 bytes from entry `at` on
+    __device__ __forceinline__ Pack fetch_at(int at) const {
+        Words w;
+        if (at + VEC <= V) {
+            w = *reinterpret_cast<const Words*>(src + at);
+        } else {
+            Pack p = fill();
+            read_end(p, at);
+            w = __builtin_bit_cast(Words, p);
+        }
+        return canonical_at(w, at);
     }
 
     __device__ __forceinline__ void open(const T* row, int count) {
