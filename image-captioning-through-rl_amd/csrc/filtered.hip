@@ -608,7 +608,8 @@ struct Kept { u64 w; unsigned index, pad; };
 // Bound by the arithmetic of the passes that weigh entries (about 45 instructions an entry, 20 of them float64; a top-p
 // over the whole row weighs it twice) and, with a list, by two reads of the row on one CU.  Measured (us a call): 1 row of
 // 10 000, top-k 50 and top-p 0.95: 10.4; 512 rows of 10 000, top-p 0.9: 31 (the rows' bytes alone take 5, the vector
-// instructions, 144 an entry altogether, 20); 333 rows of 50 257 f16, min-p 0.05: 31-34; 64 rows of 131 072 bf16, settings of their own, with the launches below: 54-61.
+// instructions, 144 an entry altogether, 20); 333 rows of 50 257 f16, min-p 0.05: 31-34; 64 rows of 131 072 bf16, settings of
+// their own, with the launches below: 54-61.
 // split.rows not null: rows that need the weights of all their entries are left to the launches that follow.
 template <typename T, int NT>
 __global__ __launch_bounds__(NT, 4) void sample_filtered_kernel(const T* __restrict__ logits, int64_t ld, int V, int S, Requests all,
