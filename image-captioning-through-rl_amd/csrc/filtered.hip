@@ -470,7 +470,8 @@ __device__ __forceinline__ float bound_of(float own_max, int k, Shared<NT>& sm) 
 
 // Composites of the entries >= bound (> -inf) into sm.hist, at most `room` of them; returns how many there are.  A thread
 // keeps its first two to itself, so that nothing waits for the shared counter while it reads; only what a thread finds
-// beyond them goes through it one by one.  FEW: hardly a vector holds any.  Otherwise a wave goes through one find of every
+// beyond them goes through it one by one.  FEW: hardly a vector holds any (the lists of a top-k; 64 rows of 131072 bf16 with
+// settings of their own, first launch: 25 us, 30 without).  Otherwise a wave goes through one find of every
 // lane at a time, as often as its busiest lane has finds, once or twice, and not once for each place of a vector (333 rows
 // of 50257 f16 with some 600 finds: 47 against 38 us; a record's 64 of 10000, 512 threads: 44.2 against 45.3, of 30000, 1024
 // threads: 82.8 against 74.5).
@@ -626,8 +627,8 @@ struct Kept { u64 w; unsigned index; float x; };
 // of those w_i >= min_p; the token is the first kept one, by index, at which the running mass exceeds u times the total.
 // Bound by the arithmetic of the passes that weigh entries (about 45 instructions an entry, 20 of them float64; a top-p
 // over the whole row weighs it twice) and, with a list, by two reads of the row on one CU.  Measured (us a call): 1 row of
-// 10 000, top-k 50 and top-p 0.95: 10.4; 512 rows of 10 000, top-p 0.9: 31 (the rows' bytes alone take 5, the vector
-// instructions, 144 an entry altogether, 20); 333 rows of 50 257 f16, min-p 0.05: 31-34; 64 rows of 131 072 bf16, settings of
+// 10 000, top-k 50 and top-p 0.95: 10.4; 512 rows of 10 000, top-p 0.9: 31-33 (the rows' bytes alone take 5, the vector
+// instructions, 144 an entry altogether, 20); 333 rows of 50 257 f16, min-p 0.05: 27; 64 rows of 131 072 bf16, settings of
 // their own, with the launches below: 54-61.
 // split.rows not null: rows that need the weights of all their entries are left to the launches that follow.
 template <typename T, int NT>
@@ -698,7 +699,7 @@ __global__ __launch_bounds__(NT, 4) void sample_filtered_kernel(const T* __restr
     if (bound > -INFINITY) {
         constexpr int ITEMS = NT >= 1024 ? 2 : 4;   // entries a thread may hold; lists that are ranked have one each
         const bool rank = by_k || by_p;
-        const int room = rank ? NT : NT * ITEMS, n = collect<NT, false>(row, sm, bound, room);
+        const int room = rank ? NT : NT * ITEMS, n = by_k ? collect<NT, true>(row, sm, bound, room) : collect<NT, false>(row, sm, bound, room);
         bool listed = n <= room;
         if (listed) {
             u64 c[ITEMS], w[ITEMS];
@@ -990,7 +991,7 @@ __global__ __launch_bounds__(CHUNK_NT, 4) void sample_chunk_draw(const T* __rest
 // ---------------------------------------------------------------------------------------------- top-k and log-normaliser
 // values, indices: the first k of the row's order; lse = log sum e^(x / T) = max / T + log sum e^((x - max) / T), whose sum
 // is float32 within a thread (some tens of terms) and float64 across them.  Bound by the one read of the row, which then
-// stays in registers: 9728 rows of 10 000 (389 MB), k = 64: 101 us, 3.9 TB/s, against 4.0 of a plain sum.  Eight waves a
+// stays in registers: 9728 rows of 10 000 (389 MB), k = 64: 101-103 us, 3.8 TB/s, against 4.0 of a plain sum.  Eight waves a
 // SIMD, four workgroups a CU, so that one row's ranking runs under the others' reads.
 template <typename T, int NT, int PLACE>
 __global__ __launch_bounds__(NT, 8) void topk_lse_kernel(const T* __restrict__ logits, int64_t ld, int V, int k, double per_t,
